@@ -100,7 +100,8 @@ VELO_API const char *velo_cuda_last_error(void);
 VELO_API int32_t velo_cuda_abi_version(void);
 
 /* Use `stream` (a cudaStream_t, may be NULL for the context's own stream) for
- * all following asynchronous work of this context. */
+ * all following asynchronous work of this context.  The device's default
+ * stream, whose handle is NULL, is named by cudaStreamLegacy ((cudaStream_t)1). */
 VELO_API int32_t velo_cuda_set_stream(velo_cuda_ctx *ctx, void *stream);
 
 /* Wait for the context's stream, giving up after timeout_ns (<0: forever).
@@ -277,6 +278,110 @@ VELO_API int32_t velo_cuda_tree_attention(velo_cuda_ctx *ctx, const void *q, con
                                           int32_t n_nodes, int32_t n_head, int32_t n_kv,
                                           int32_t head_dim, int32_t kv_dtype, void *out,
                                           int32_t out_dtype);
+
+/* ---- one-token decoding over a caller's paged cache ----------------------- */
+
+/* Element types of activations and logits rows. */
+typedef enum velo_elem { VELO_ELEM_F32 = 0, VELO_ELEM_F16 = 1, VELO_ELEM_BF16 = 2 } velo_elem;
+
+/* A paged KV cache that the caller owns (all pointers device memory on the
+ * context's GPU, pools and scales 16-byte aligned): one layer's pages, in the
+ * layout of velo_cuda_tree_attention.
+ *   k_pool, v_pool   [pool_pages][n_kv][16][head_dim]: f16 (VELO_KV_F16), int8
+ *                    (VELO_KV_INT8, value = q * scale) or f32 (VELO_KV_F32)
+ *   k_scale, v_scale [pool_pages][n_kv][16] f16 (INT8 only, else NULL)
+ *   page_table       [rows][max_pages] u32 page ids: row b belongs to sequence b
+ * head_dim 64 or 128. */
+typedef struct velo_kv_cache {
+    uint32_t struct_size;  /* sizeof(velo_kv_cache) */
+    int32_t kv_dtype;      /* velo_kv_dtype */
+    void *k_pool, *v_pool;
+    void *k_scale, *v_scale;
+    const uint32_t *page_table;
+    int32_t pool_pages, max_pages, n_kv, head_dim;
+} velo_kv_cache;
+
+/* Append the K/V rows of new tokens to the cache, rotated to their positions on
+ * the way, and rotate their queries (RoPE of the verify step: NeoX half split,
+ * llama_cpu.rs:98-132; the angles are reduced exactly, so far positions keep
+ * their precision).  Device memory, asynchronous on the context stream.
+ *   q [n_tokens][n_head][head_dim], k and v [n_tokens][n_kv][head_dim]: elements
+ *             of in_dtype (velo_elem); token t's row starts at t * ldq / ldk /
+ *             ldv elements, so all three may be slices of one projection's
+ *             output.  Rows 16-byte aligned.  Without q: q and q_out NULL, n_head 0.
+ *   seq_start [B+1] i32, non-decreasing: tokens seq_start[b] ..
+ *             seq_start[b+1] - 1 continue sequence b; rows from seq_start[B] on
+ *             are padding (nothing is read or written for them).  NULL: token t
+ *             is sequence t's only one (n_tokens == B).
+ *   ctx_len   [B] i32 tokens cached before the call: token t of sequence b goes
+ *             to position ctx_len[b] + t - seq_start[b].
+ *   q_out     [n_tokens][n_head][head_dim], f32 for f32 pages, else f16
+ *   k_out, v_out  [n_tokens][n_kv][head_dim] (type of q_out; both or NULL): the rows
+ *             as the cache now holds them (INT8: q * scale), for attention
+ *             among the new tokens (node_k / node_v of velo_cuda_tree_attention)
+ * f16 and f32 pages take the rotated value rounded once; INT8 pages quantise it
+ * as velo_cuda_write_kv does (scale = f16(max|x| / 127), truncation).  A
+ * position past the page-table row, a page id outside the pool or a negative
+ * ctx_len sets the device flag (velo_cuda_sync); that token's K/V are not
+ * written.  Page-table rows must not share the pages written here.  Replaces
+ * kv_update / kv_update_int8 (src/kernels.metal:619-645, 753-802) after the
+ * per-head rope of forward_one (src/llama_cpu.rs:113-132). */
+VELO_API int32_t velo_cuda_kv_append(velo_cuda_ctx *ctx, const velo_kv_cache *cache, const void *q,
+                                     const void *k, const void *v, int32_t in_dtype, int64_t ldq,
+                                     int64_t ldk, int64_t ldv, const int32_t *seq_start,
+                                     const int32_t *ctx_len, int32_t B, int32_t n_tokens,
+                                     int32_t n_head, float freq_base, void *q_out, void *k_out,
+                                     void *v_out);
+
+/* Device bytes of the workspace velo_cuda_decode_attention needs (any B and any
+ * lengths) for these head counts; 0 for arguments that call refuses. */
+VELO_API size_t velo_cuda_decode_attention_workspace(velo_cuda_ctx *ctx, int32_t n_head, int32_t n_kv,
+                                                     int32_t head_dim);
+
+/* Attention of one query token per sequence over its cached tokens.  Device
+ * memory, asynchronous on the context stream; allocates nothing.
+ *   q         [B][n_head][head_dim] (RoPE applied), f32 for f32 pages, else f16;
+ *             sequence b's row starts at b * ldq elements
+ *   seq_len   [B] i32: sequence b attends to positions 0 .. seq_len[b] - 1 (its
+ *             own new token included, once appended)
+ *   scale     of the scores; 0: 1 / sqrt(head_dim)
+ *   out       [B][n_head][head_dim], type of q, dense
+ *   lse       [B][n_head] f32: log of the sum of the exponentials of the scaled
+ *             scores, to join this result with another's (or NULL)
+ *   workspace scratch of velo_cuda_decode_attention_workspace bytes, 16-byte
+ *             aligned, contents free; calls that may overlap (other streams,
+ *             graphs replayed at once) need one each
+ * A sequence of length 0 gives out = 0 and lse = -inf.  GQA: head h reads KV head
+ * h / (n_head / n_kv).  Slots past seq_len in the last page are never used,
+ * whatever they hold.  A negative or too long seq_len (clamped to the
+ * page-table row) and a page id outside the pool (its tokens are left out) set
+ * the device flag (velo_cuda_sync).  B <= 4096.  Repeated calls give the same
+ * bits.  Replaces paged_attention_flash (src/kernels.metal:440-501, 672-732);
+ * velo_cuda_tree_attention serves draft trees. */
+VELO_API int32_t velo_cuda_decode_attention(velo_cuda_ctx *ctx, const velo_kv_cache *cache, const void *q,
+                                            int64_t ldq, const int32_t *seq_len, int32_t B,
+                                            int32_t n_head, float scale, void *out, float *lse,
+                                            void *workspace, size_t workspace_bytes);
+
+/* Log probability of given tokens under softmax(logits / temperature), with the
+ * distribution's entropy (nats) and its best alternatives.  Device memory,
+ * asynchronous on the context stream.
+ *   logits    [M][V] of logits_dtype (velo_elem), row m at m * ldl elements
+ *   tokens    [M] u32 (NULL: no logprob)
+ *   logprob   [M] f32 (with tokens), entropy [M] f32 (or NULL)
+ *   top_tokens [M][n_top] u32, top_logprobs [M][n_top] f32: the n_top largest
+ *             logits in descending order, the lower index first among equal
+ *             ones (n_top <= 64 and <= V; 0: neither)
+ * Entries of -inf (masked) have probability 0; a row of -inf alone gives logprob
+ * -inf and entropy 0.  NaN or +inf anywhere in a row makes its logprobs and
+ * entropy NaN; top_tokens rank NaN below -inf.  A token >= V gives NaN and sets
+ * the device flag (velo_cuda_sync).  The reference computes no log
+ * probabilities: the host would take them from CausalLmBackend's logits
+ * (src/backend.rs:313-369). */
+VELO_API int32_t velo_cuda_token_logprobs(velo_cuda_ctx *ctx, const void *logits, int32_t logits_dtype,
+                                          int64_t ldl, int32_t M, int32_t V, const uint32_t *tokens,
+                                          float temperature, float *logprob, float *entropy,
+                                          int32_t n_top, uint32_t *top_tokens, float *top_logprobs);
 
 /* ---- model, KV pages and the verify step -------------------------------- */
 

@@ -1,0 +1,164 @@
+// kv_append.cu -- new K/V rows into the paged cache, rotated to their positions
+// on the way, with the rotated queries (velo_cuda_kv_append).
+//
+// rot(x)_i = x_i cos a - x_{i+D/2} sin a, rot(x)_{i+D/2} = x_i sin a + x_{i+D/2} cos a,
+// a = pos * base^(-2i/D).  An angle in f32 loses all its digits far into a long
+// context (pos 10^5 leaves 2^-7 of a radian), so the frequency is kept in turns
+// as a 64-bit fraction and pos * f wraps modulo one turn by itself; only the
+// remainder in [-1/2, 1/2) turns becomes an f32.
+//
+// One block per token: its angles are computed once (a thread per pair) into
+// shared memory, then a thread takes 8 rotation pairs of a head.
+#include "common/elem.cuh"
+#include "kernels/decode_ops.h"
+#include "velo_cuda.h"
+
+namespace velo {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kErrAppend = 0x6201;
+
+// Number of sequences that start at or before token t, minus one: its sequence
+// (the last of several that start at the same token, so empty ones are passed
+// over).  A two-level search over blockDim sorted starts each.
+__device__ __forceinline__ int find_sequence(const int32_t* start, int B, int t) {
+    int lo = 0, n = B;  // the answer lies in [lo, lo + n)
+    while (n > 1) {
+        const int step = (n + (int)blockDim.x - 1) / (int)blockDim.x;
+        const int i = (int)threadIdx.x * step;
+        const int hit = __syncthreads_count(i < n && start[lo + i] <= t);
+        if (hit == 0) return -1;
+        lo += (hit - 1) * step;
+        n = min(step, n - (hit - 1) * step);
+    }
+    return lo;
+}
+
+template <typename In, typename Act, typename Kv, int D>
+__global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs a) {
+    constexpr int kLanes = D / 16;  // threads per head, 8 pairs each
+    __shared__ float cs[D / 2], sn[D / 2];
+    const int t = blockIdx.x;
+    int b = t, first = t;
+    if (a.seq_start) {
+        if (t >= a.seq_start[a.B]) return;  // padding rows
+        b = find_sequence(a.seq_start, a.B, t);
+        if (b >= 0) first = a.seq_start[b];
+        if (b < 0 || first > t || t >= a.seq_start[b + 1]) {
+            if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrAppend);
+            return;
+        }
+    }
+    const int cached = a.ctx_len[b];
+    const long long pos = (long long)cached + (t - first);
+    const int pi = (int)(pos / kPageTokens), slot = (int)(pos % kPageTokens);
+    bool ok = cached >= 0 && pos / kPageTokens < a.kv.max_pages;
+    uint32_t page = 0;
+    if (ok) {
+        page = a.kv.page_table[(size_t)b * a.kv.max_pages + pi];
+        ok = page < (uint32_t)a.kv.pool_pages;
+    }
+    if (!ok && threadIdx.x == 0) atomicCAS(a.err, 0, kErrAppend);
+    if (threadIdx.x < D / 2) {
+        const uint64_t turn = (uint64_t)pos * a.turns.f[threadIdx.x];
+        // the upper 32 bits as a signed fraction of a turn; sincospi takes half turns
+        const float half_turns = (float)(int32_t)(turn >> 32) * 4.656612873077393e-10f;  // 2^-31
+        sincospif(half_turns, &sn[threadIdx.x], &cs[threadIdx.x]);
+    }
+    __syncthreads();
+    const int Hkv = a.kv.n_kv, heads = a.Hq + 2 * Hkv;
+    for (int w = threadIdx.x; w < (heads * kLanes + 31) / 32 * 32; w += kThreads) {
+        const int hh = w / kLanes, i0 = (w % kLanes) * 8;
+        const bool live = hh < heads, is_q = hh < a.Hq, is_v = hh >= a.Hq + Hkv;
+        const int h = is_q ? hh : is_v ? hh - a.Hq - Hkv : hh - a.Hq;
+        float x0[8], x1[8];
+        if (live) {
+            const In* src = static_cast<const In*>(is_q ? a.q : is_v ? a.v : a.k) +
+                            (size_t)t * (is_q ? a.ldq : is_v ? a.ldv : a.ldk) + (size_t)h * D;
+            load8(src + i0, x0);
+            load8(src + i0 + D / 2, x1);
+            if (!is_v) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float c = cs[i0 + e], s = sn[i0 + e];
+                    const float r0 = x0[e] * c - x1[e] * s, r1 = x0[e] * s + x1[e] * c;
+                    x0[e] = r0;
+                    x1[e] = r1;
+                }
+            }
+            if (is_q) {
+                Act* dst = static_cast<Act*>(a.q_out) + ((size_t)t * a.Hq + h) * D;
+                store8(dst + i0, x0);
+                store8(dst + i0 + D / 2, x1);
+            }
+        }
+        const size_t row = ((size_t)page * Hkv + h) * kPageTokens + slot;
+        void* pool = is_v ? a.kv.v_pool : a.kv.k_pool;
+        if constexpr (sizeof(Kv) == 1) {  // quantise: the head's lanes share the maximum
+            float mx = 0.0f;
+            if (live) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) mx = fmaxf(mx, fmaxf(fabsf(x0[e]), fabsf(x1[e])));
+            }
+#pragma unroll
+            for (int o = kLanes / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            if (!live || is_q) continue;
+            const float inv = mx > 0.0f ? __fdiv_rn(127.0f, mx) : 0.0f;
+            const __half scale = __float2half_rn(__fdiv_rn(mx, 127.0f));
+            uint32_t w0[2] = {0, 0}, w1[2] = {0, 0};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int q0 = (int)__fmul_rn(x0[e], inv), q1 = (int)__fmul_rn(x1[e], inv);  // truncation
+                w0[e / 4] |= (uint32_t)(q0 & 0xff) << (8 * (e % 4));
+                w1[e / 4] |= (uint32_t)(q1 & 0xff) << (8 * (e % 4));
+                x0[e] = (float)q0 * __half2float(scale);
+                x1[e] = (float)q1 * __half2float(scale);
+            }
+            if (ok) {
+                int8_t* dst = static_cast<int8_t*>(pool) + row * D;
+                *reinterpret_cast<uint2*>(dst + i0) = make_uint2(w0[0], w0[1]);
+                *reinterpret_cast<uint2*>(dst + i0 + D / 2) = make_uint2(w1[0], w1[1]);
+                if (i0 == 0) (is_v ? a.kv.v_scale : a.kv.k_scale)[row] = scale;
+            }
+        } else {
+            if (!live || is_q) continue;
+            if (ok) {
+                Kv* dst = static_cast<Kv*>(pool) + row * D;
+                store8(dst + i0, x0);
+                store8(dst + i0 + D / 2, x1);
+            }
+        }
+        if (a.k_out) {
+            Act* dst = static_cast<Act*>(is_v ? a.v_out : a.k_out) + ((size_t)t * Hkv + h) * D;
+            store8(dst + i0, x0);
+            store8(dst + i0 + D / 2, x1);
+        }
+    }
+}
+
+template <typename In, typename Act, typename Kv>
+cudaError_t launch_typed(const KvAppendArgs& a, cudaStream_t s) {
+    if (a.kv.head_dim == 64)
+        kv_append_kernel<In, Act, Kv, 64><<<a.T, kThreads, 0, s>>>(a);
+    else
+        kv_append_kernel<In, Act, Kv, 128><<<a.T, kThreads, 0, s>>>(a);
+    return cudaGetLastError();
+}
+
+template <typename In>
+cudaError_t launch_from(const KvAppendArgs& a, cudaStream_t s) {
+    if (a.kv.kv_dtype == VELO_KV_F32) return launch_typed<In, float, float>(a, s);
+    if (a.kv.kv_dtype == VELO_KV_INT8) return launch_typed<In, __half, int8_t>(a, s);
+    return launch_typed<In, __half, __half>(a, s);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const KvAppendArgs& a, int, cudaStream_t s) {
+    if (a.in_dtype == VELO_ELEM_F32) return launch_from<float>(a, s);
+    if (a.in_dtype == VELO_ELEM_F16) return launch_from<__half>(a, s);
+    return launch_from<__nv_bfloat16>(a, s);
+}
+
+}  // namespace velo

@@ -75,6 +75,9 @@ struct velo_cuda_ctx {
     velo::DeviceBuffer attn_ws;    // tree attention: ancestor masks
     int* err_flag = nullptr;       // device-side input flag
     int* err_host = nullptr;       // pinned host copy of err_flag (read at sync)
+    float rope_base = 0.0f;        // rotation table of kv_append, of the last (base, head_dim)
+    int rope_dim = 0;
+    uint64_t rope_turns[64] = {};
     velo::Model* model = nullptr;  // weights, KV pool and verify buffers (velo_cuda_load_model)
     void* nccl_comm = nullptr;     // ncclComm_t of the tensor-parallel group (tp_size > 1)
     void* nccl_comm2 = nullptr;    // a second communicator of the group (ncclCommSplit), so

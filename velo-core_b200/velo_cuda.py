@@ -39,6 +39,8 @@ ERR_MISSING_TENSOR = 17
 ERR_INVALID_SHAPE = 18
 
 KV_F16, KV_INT8, KV_F32 = 0, 1, 2  # KV_F32: the fp32 path of the model
+ELEM_F32, ELEM_F16, ELEM_BF16 = 0, 1, 2  # velo_elem
+DEFAULT_STREAM = 1  # cudaStreamLegacy: Context.set_stream's name for the device's default stream
 
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
@@ -100,6 +102,13 @@ _SIGS = {
     "velo_cuda_gemm_q4_0": (_I32, [_P, _P, _P, _I32, _I32, _I32, _P, _I32, _I32]),
     "velo_cuda_tree_attention": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P,
                                         _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32]),
+    "velo_cuda_kv_append": (_I32, [_P, _P, _P, _P, _P, _I32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, _P,
+                                   _I32, _I32, _I32, ctypes.c_float, _P, _P, _P]),
+    "velo_cuda_decode_attention_workspace": (_SZ, [_P, _I32, _I32, _I32]),
+    "velo_cuda_decode_attention": (_I32, [_P, _P, _P, ctypes.c_int64, _P, _I32, _I32, ctypes.c_float, _P, _P, _P,
+                                          _SZ]),
+    "velo_cuda_token_logprobs": (_I32, [_P, _P, _I32, ctypes.c_int64, _I32, _I32, _P, ctypes.c_float, _P, _P, _I32,
+                                        _P, _P]),
     "velo_cuda_load_model": (_I32, [_P, _P, _P, _I32]),
     "velo_cuda_bind_slot": (_I32, [_P, ctypes.c_uint32, _P, ctypes.c_size_t]),
     "velo_cuda_write_kv": (_I32, [_P, ctypes.c_uint32, _I32, _I32, _I32, _P, _P]),
@@ -172,6 +181,12 @@ class WeightDesc(ctypes.Structure):
 WEIGHT_DEVICE, WEIGHT_SHARD = 1, 2
 
 
+class KvCacheDesc(ctypes.Structure):
+    _fields_ = [("struct_size", ctypes.c_uint32), ("kv_dtype", _I32), ("k_pool", _P), ("v_pool", _P),
+                ("k_scale", _P), ("v_scale", _P), ("page_table", _P), ("pool_pages", _I32), ("max_pages", _I32),
+                ("n_kv", _I32), ("head_dim", _I32)]
+
+
 class VerifyBatch(ctypes.Structure):
     _fields_ = [("struct_size", ctypes.c_uint32), ("B", ctypes.c_int32), ("n_nodes", ctypes.c_int32),
                 ("slots", _P), ("ctx_len", _P), ("tokens", _P), ("parents", _P),
@@ -232,6 +247,69 @@ def _ptr(a):
     return ctypes.c_void_p(a.data_ptr())  # torch tensor
 
 
+_ELEMS = {"torch.float32": ELEM_F32, "torch.float16": ELEM_F16, "torch.bfloat16": ELEM_BF16}
+_KVS = {"torch.float16": KV_F16, "torch.int8": KV_INT8, "torch.float32": KV_F32}
+
+
+def _refuse(message):
+    raise VeloError(ERR_INVALID_ARGUMENT, message)
+
+
+def _tensor(what, t, dtypes, shape, device, strided=False):
+    """Refuse a tensor of another element type, shape, device or layout (strided:
+    the first dimension may have any stride, the others are dense).  Returns
+    its address."""
+    if t is None:
+        _refuse(f"{what} is missing")
+    if str(t.dtype) not in dtypes:
+        _refuse(f"{what}: {t.dtype}, not {' / '.join(dtypes)}")
+    if t.shape != shape:
+        _refuse(f"{what}: shape {tuple(t.shape)}, not {shape}")
+    if t.get_device() != device:
+        _refuse(f"{what}: on {t.device}, not on the context's device {device}")
+    if not t.is_contiguous():
+        dense, step = strided, 1
+        for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
+            dense = dense and (st == step or n == 1)
+            step *= n
+        if not dense:
+            _refuse(f"{what}: strides {t.stride()} unsupported")
+    return t.data_ptr()
+
+
+_INTS, _FLOAT = ("torch.int32", "torch.uint32"), ("torch.float32",)
+
+
+class KvCache:
+    """velo_kv_cache over torch CUDA tensors: pools [pages][n_kv][16][head_dim]
+    (f16, int8 or f32), page_table [rows][max_pages] int32 and, for int8, scales
+    [pages][n_kv][16] f16.  Keeps the tensors alive; their contents may change
+    between calls."""
+
+    def __init__(self, k_pool, v_pool, page_table, k_scale=None, v_scale=None):
+        if k_pool.dim() != 4 or k_pool.shape[2] != 16:
+            _refuse(f"k_pool: shape {tuple(k_pool.shape)}, not [pages][n_kv][16][head_dim]")
+        if page_table.dim() != 2:
+            _refuse(f"page_table: shape {tuple(page_table.shape)}, not [rows][max_pages]")
+        pages, n_kv, _, hd = k_pool.shape
+        dev = self.device = k_pool.get_device()
+        kp = _tensor("k_pool", k_pool, _KVS, k_pool.shape, dev)
+        vp = _tensor("v_pool", v_pool, (str(k_pool.dtype),), k_pool.shape, dev)
+        tb = _tensor("page_table", page_table, _INTS, page_table.shape, dev)
+        self.kv_dtype, sp = _KVS[str(k_pool.dtype)], [None, None]
+        if self.kv_dtype == KV_INT8:
+            if k_scale is None or v_scale is None:
+                _refuse("int8 pools need k_scale and v_scale")
+            sp = [_tensor(w, t, ("torch.float16",), k_pool.shape[:3], dev)
+                  for w, t in (("k_scale", k_scale), ("v_scale", v_scale))]
+        self.act = "torch.float32" if self.kv_dtype == KV_F32 else "torch.float16"
+        self.rows, self.n_kv, self.head_dim = page_table.shape[0], n_kv, hd
+        self.tensors = (k_pool, v_pool, page_table, k_scale, v_scale)
+        self.desc = KvCacheDesc(ctypes.sizeof(KvCacheDesc), self.kv_dtype, kp, vp, sp[0], sp[1], tb, pages,
+                                page_table.shape[1], n_kv, hd)
+        self.ref = ctypes.byref(self.desc)
+
+
 class Context:
     """One velo_cuda_ctx: a device, a stream and the device buffers."""
 
@@ -266,6 +344,8 @@ class Context:
         return self._h
 
     def set_stream(self, stream_ptr):
+        """Stream of the following asynchronous work (a cudaStream_t; 0 or None: the
+        context's own; DEFAULT_STREAM: the device's default stream)."""
         check(lib().velo_cuda_set_stream(self._h, _P(stream_ptr) if stream_ptr else None))
 
     def sync(self, timeout_ns=-1):
@@ -343,6 +423,85 @@ class Context:
             k_pool.shape[0], _ptr(page_table), page_table.shape[1], _ptr(ctx_len), _ptr(node_k),
             _ptr(node_v), _ptr(parents), B, N, Hq, n_kv, hd, kv_dtype, _ptr(out), out_f16))
 
+
+    # ------------------------------------------------------------ one-token decoding
+    def kv_append(self, cache, q, k, v, ctx_len, q_out, freq_base, seq_start=None, k_out=None, v_out=None):
+        """Append new tokens' rotated K and V to `cache` and rotate their queries
+        (torch CUDA tensors, asynchronous).  q [T][n_head][hd] (or None, with
+        q_out), k, v [T][n_kv][hd] f32 / f16 / bf16, rows of any stride; ctx_len
+        [B] int32 cached tokens; seq_start [B+1] int32 (None: one token per
+        sequence); outputs f32 for f32 pools, else f16."""
+        n, hd, dev, e = cache.n_kv, cache.head_dim, self.device, (str(k.dtype),)
+        T, B = k.shape[0], ctx_len.shape[0]
+        if cache.device != dev or cache.rows < B:
+            _refuse(f"cache: device {cache.device}, {cache.rows} page-table rows for {B} sequences on device {dev}")
+        if e[0] not in _ELEMS:
+            _refuse(f"k: {k.dtype}, not {' / '.join(_ELEMS)}")
+        pq = pqo = pko = pvo = pss = None
+        ldq = Hq = 0
+        if q is not None:
+            Hq = q.shape[1]
+            pq, ldq = _tensor("q", q, e, (T, Hq, hd), dev, True), max(q.stride(0), Hq * hd) if T < 2 else q.stride(0)
+            pqo = _tensor("q_out", q_out, (cache.act,), (T, Hq, hd), dev)
+        pk, pv = _tensor("k", k, e, (T, n, hd), dev, True), _tensor("v", v, e, (T, n, hd), dev, True)
+        ldk, ldv = (k.stride(0), v.stride(0)) if T > 1 else (n * hd, n * hd)
+        if k_out is not None or v_out is not None:
+            pko = _tensor("k_out", k_out, (cache.act,), (T, n, hd), dev)
+            pvo = _tensor("v_out", v_out, (cache.act,), (T, n, hd), dev)
+        if seq_start is not None:
+            pss = _tensor("seq_start", seq_start, ("torch.int32",), (B + 1,), dev)
+        check(lib().velo_cuda_kv_append(
+            self._h, cache.ref, pq, pk, pv, _ELEMS[e[0]], ldq, ldk, ldv, pss,
+            _tensor("ctx_len", ctx_len, ("torch.int32",), (B,), dev), B, T, Hq, freq_base, pqo, pko, pvo))
+
+    def decode_attention_workspace(self, n_head, n_kv, head_dim):
+        """Bytes of decode_attention's workspace, for any batch and lengths."""
+        n = lib().velo_cuda_decode_attention_workspace(self._h, n_head, n_kv, head_dim)
+        if n == 0:
+            _refuse(f"decode_attention: n_head {n_head}, n_kv {n_kv}, head_dim {head_dim}")
+        return n
+
+    def decode_attention(self, cache, q, seq_len, out, workspace, lse=None, scale=0.0):
+        """Attention of one query token per sequence over `cache` (torch CUDA
+        tensors, asynchronous).  q [B][n_head][hd] (rows of any stride) and out
+        f32 for f32 pools, else f16; seq_len [B] int32; lse [B][n_head] f32;
+        workspace: a tensor of decode_attention_workspace bytes."""
+        B, Hq, hd = shape = q.shape
+        dev = self.device
+        if cache.device != dev or cache.rows < B or cache.head_dim != hd:
+            _refuse(f"cache: device {cache.device}, {cache.rows} page-table rows, head_dim {cache.head_dim} for q "
+                    f"{tuple(shape)} on device {dev}")
+        pq = _tensor("q", q, (cache.act,), shape, dev, True)
+        po = _tensor("out", out, (cache.act,), shape, dev)
+        pl = None if lse is None else _tensor("lse", lse, _FLOAT, (B, Hq), dev)
+        pw = _tensor("workspace", workspace, (str(workspace.dtype),), workspace.shape, dev)
+        check(lib().velo_cuda_decode_attention(
+            self._h, cache.ref, pq, q.stride(0) if B > 1 else Hq * hd,
+            _tensor("seq_len", seq_len, ("torch.int32",), (B,), dev), B, Hq, scale, po, pl, pw, workspace.nbytes))
+
+    def token_logprobs(self, logits, tokens, logprob, entropy=None, top_tokens=None, top_logprobs=None,
+                       temperature=1.0):
+        """Log probabilities of `tokens` [M] (int32; None with logprob None) under
+        softmax(logits / temperature), logits [M][V] f32 / f16 / bf16 with rows of
+        any stride, with the entropy [M] and the n best alternatives, top_tokens
+        (int32) and top_logprobs [M][n] (torch CUDA tensors, asynchronous)."""
+        M, V = shape = logits.shape
+        dev = self.device
+        px = _tensor("logits", logits, _ELEMS, shape, dev, True)
+        pt = pl = pe = ptt = ptl = None
+        n = 0
+        if tokens is not None or logprob is not None:
+            pt = _tensor("tokens", tokens, _INTS, (M,), dev)
+            pl = _tensor("logprob", logprob, _FLOAT, (M,), dev)
+        if entropy is not None:
+            pe = _tensor("entropy", entropy, _FLOAT, (M,), dev)
+        if top_tokens is not None or top_logprobs is not None:
+            n = top_tokens.shape[1] if top_tokens is not None else 0
+            ptt = _tensor("top_tokens", top_tokens, _INTS, (M, n), dev)
+            ptl = _tensor("top_logprobs", top_logprobs, _FLOAT, (M, n), dev)
+        check(lib().velo_cuda_token_logprobs(
+            self._h, px, _ELEMS[str(logits.dtype)], logits.stride(0) if M > 1 else V, M, V, pt, temperature, pl, pe, n,
+            ptt, ptl))
 
     # ------------------------------------------------------------ model + verify
     def load_model(self, meta, tensors, shards=False):
