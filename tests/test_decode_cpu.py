@@ -42,3 +42,75 @@ def test_turn_fractions_keep_far_angles(base, D):
             exact = np.longdouble(pos) * np.longdouble(base) ** (np.longdouble(-2 * i) / D) / np.longdouble(np.pi)
             off = (np.longdouble(half) - exact) % 2
             assert min(off, 2 - off) <= 2.0 ** -23
+
+
+def _ranges(units, per_seq, blocks, whole=16, least=4):
+    """decode_attn.cu's cut of the unit list: per block its pieces (item, first,
+    last + 1 unit of the item), the slot of each partial piece, and the open
+    item's last block."""
+    pre = np.concatenate(([0], np.cumsum(np.asarray(units) * per_seq)))
+    total = int(pre[-1])
+    blocks = min(blocks, -(-total // least))
+
+    def item(u):
+        b = int(np.searchsorted(pre, u, "right")) - 1
+        n = int(pre[b + 1] - pre[b]) // per_seq
+        it = int(u - pre[b]) // n
+        return (b, it), int(pre[b]) + it * n, n
+
+    def cut(c):
+        u = total * c // blocks
+        if c == 0 or u >= total:
+            return u
+        _, start, n = item(u)
+        return start if n <= max(whole, total // blocks // 4) else u
+    out = []
+    for c in range(blocks):
+        seg, u1 = cut(c), cut(c + 1)
+        pieces, open_ = [], None
+        while seg < u1:
+            key, start, n = item(seg)
+            end, stop = start + n, min(start + n, u1)
+            full = seg == start and stop == end
+            pieces.append((key, seg - start, stop - start, n, None if full else 2 * c + (seg == start)))
+            if not full and seg == start:
+                assert open_ is None
+                open_ = (key, (end * blocks - 1) // total)
+            seg = stop
+        out.append((pieces, open_))
+    return out
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_decode_work_list_covers_every_item_once(seed):
+    """Every unit of every item is in exactly one block; an item cut between
+    blocks is open in its first one, whose join reads slot 1 of that block and
+    slot 0 of the following ones, each written once."""
+    rng = np.random.default_rng(seed)
+    B = int(rng.integers(1, 30))
+    units = rng.integers(0, int(rng.choice([2, 20, 500])), B)
+    if not units.any():
+        units[0] = 1
+    per_seq, blocks = int(rng.choice([1, 2, 8, 32])), int(rng.choice([1, 7, 296]))
+    out = _ranges(units, per_seq, blocks)
+    got, written = {}, {}
+    for pieces, _ in out:
+        for key, lo, hi, n, slot in pieces:
+            assert n == units[key[0]] and lo < hi
+            got.setdefault(key, []).append((lo, hi))
+            if slot is not None:
+                assert slot not in written
+                written[slot] = (key, lo)
+    assert set(got) == {(b, i) for b in range(B) if units[b] for i in range(per_seq)}
+    for key, parts in got.items():
+        assert parts[0][0] == 0 and parts[-1][1] == units[key[0]]
+        assert all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+    read = []
+    for c, (_, open_) in enumerate(out):
+        if open_:
+            key, last = open_
+            states = [2 * c + 1] + [2 * i for i in range(c + 1, last + 1)]
+            assert [written.get(s, (None,))[0] for s in states] == [key] * len(states)
+            assert [written[s][1] for s in states] == [p[0] for p in got[key]]
+            read += states
+    assert sorted(read) == sorted(written)

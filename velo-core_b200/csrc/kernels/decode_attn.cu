@@ -1,96 +1,816 @@
 // decode_attn.cu -- attention of one query token per sequence over the paged
 // cache (velo_cuda_decode_attention).
 //
-// One block of four warps per (sequence, head): warp w takes tokens w, w + 4,
-// ...; a lane holds D / 32 dimensions of q and of the running output; online
-// softmax per warp, the four states merged through shared memory.
+// s_j = scale q.k_j, p = softmax(s), out = sum p_j v_j: every K and V byte is used
+// once per KV head by its few query heads (4 flop per element and head), so HBM
+// bounds it and the matrix work only has to stay out of the way.
+//
+// Work: the batch is one list of units -- a unit is a step of 16 (f16), 32 (int8)
+// or 8 (f32) tokens of one item, an item a (sequence, KV head, tile of query
+// heads) -- cut into equal ranges, one per block, two blocks per SM, whatever the
+// lengths are.  An item that a cut runs through leaves partial states (max, sum,
+// unnormalised output) in the workspace, which the join kernel, launched as a
+// programmatic dependent, adds in order: no atomics, repeatable bits.  Short
+// items are not cut (the cut moves to their start), so a batch of short contexts
+// pays no join.
+//
+// A block's four warps take the units of its range in turn.  Each warp streams
+// its own units through a private ring of 8 KB (head_dim 128) stages filled by
+// 16-byte cp.async (three stages: 96 KB in flight per block), so no block-wide
+// barrier stands between the loads and the arithmetic; tokens past the length are
+// zero-filled, never read.  Query heads of a KV head are the rows of mma.sync
+// tiles (m16n8k16; tcgen05's 128-row tiles would be 1/16 full at 8 heads a KV head).
+//
+//  f16: K and V fragments by ldmatrix from XOR-swizzled rows.  P is split into
+//   two f16 parts (value and remainder), so that it adds no rounding of its own:
+//   with at most 8 heads the parts fill the tile's upper and lower rows.
+//  int8: fragments are read as 16 consecutive bytes per lane (the contraction
+//   order is free, q is permuted to match); K becomes f16 and V bf16, both exact;
+//   the K scale multiplies the score and the V scale the weight, in f32.  P is
+//   split into two bf16 parts, whose exponent holds any scale.
+//  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
+//   dimensions for the output.
+#include <algorithm>
+#include <type_traits>
+
 #include "common/elem.cuh"
+#include "common/sm100.cuh"
+#include "common/smem_attr.cuh"
 #include "kernels/decode_ops.h"
 #include "velo_cuda.h"
 
 namespace velo {
 namespace {
 
+using sm100::ex2_approx;
+using sm100::smem_u32;
+
 constexpr int kErrSeqLen = 0x6211, kErrPage = 0x6212;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kBlocksPerSm = 2;
+constexpr int kMaxBlocks = 1024;
+constexpr int kMinUnits = 4;  // units per block at least: one per warp
+// An item of at most this many units (256 tokens of f16 pages), or of a quarter of
+// a block's range, is never cut.
+constexpr int kWholeUnits = 16;
+constexpr int kRing = 64;  // unit descriptions per warp
 
-template <typename Act, typename Kv, int D>
-__global__ void __launch_bounds__(128) decode_attn_kernel(const DecodeAttnArgs a) {
-    constexpr int R = D / 32;
-    __shared__ float sm[4], sl[4], so[4][D];
-    const int b = blockIdx.x / a.Hq, h = blockIdx.x % a.Hq;
-    const int Hkv = a.kv.n_kv, hk = h / (a.Hq / Hkv);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int len = a.seq_len[b];
-    if (len < 0 || len > a.kv.max_pages * kPageTokens) {
-        if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrSeqLen);
-        len = len < 0 ? 0 : a.kv.max_pages * kPageTokens;
+constexpr int tokens_of(int kv) { return kv == VELO_KV_F16 ? 16 : kv == VELO_KV_INT8 ? 32 : 8; }
+constexpr int bytes_of(int kv) { return kv == VELO_KV_F16 ? 2 : kv == VELO_KV_INT8 ? 1 : 4; }
+
+// Shared memory of a block; the lengths and the prefix sums follow.
+template <int KV, int D>
+struct Layout {
+    static constexpr int kTok = tokens_of(KV);
+    static constexpr int kRow = D * bytes_of(KV);               // bytes of a token's K or V
+    static constexpr int kHalf = kTok * kRow;                   // K, then V
+    static constexpr int kStage = 2 * kHalf + (KV == VELO_KV_INT8 ? 4 * kTok : 0);  // + scales
+    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kRings = kWarps * kStages * kStage;
+    static constexpr int kStats = kRings + kWarps * kRing * 16;
+    static constexpr int kQ = kStats + 3 * kWarps * 16 * 4;     // f32: q, and each warp's weights
+    static constexpr int kP = kQ + (KV == VELO_KV_F32 ? 8 * D * 4 : 0);
+    static constexpr int kLens = kP + (KV == VELO_KV_F32 ? kWarps * 72 * 4 : 0);
+};
+
+struct Plan {
+    int blocks;   // of the grid
+    int group;    // query heads per KV head
+    int tiles;    // query-head tiles per KV head
+};
+
+// A partial state: rows x (max, sum), then rows x D of output.
+__host__ __device__ inline size_t slot_floats(int rows, int D) { return (size_t)rows * (D + 2); }
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two f32 as a pair of 16-bit parts and the pair of their remainders.
+__device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(x, y);
+    const float2 f = __half22float2(h);
+    const __half2 r = __floats2half2_rn(x - f.x, y - f.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(x - __bfloat162float(h.x), y - __bfloat162float(h.y));
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// Bytes 2i and 2i + 1 of w (int8 with the sign bit flipped) as an exact f16
+// pair: 0x6400 | u is 1024 + u.
+template <int i>
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
+    uint32_t v = __byte_perm(w, 0x64646464u, i ? 0x4342 : 0x4140);
+    const uint32_t bias = 0x64806480u;  // 1152
+    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// Bytes b of the words w0 and w1 (int8) as an exact bf16 pair: 0x4300 | low 7
+// bits is 128 + them, 0x4300 | sign bit is 128 or 256.
+template <int b>
+__device__ __forceinline__ uint32_t byte_pair_to_bf16(uint32_t w0, uint32_t w1) {
+    const uint32_t e = __byte_perm(w0, w1, b | (4 + b) << 4);  // bytes: w0.b, w1.b, w0.0, w0.0
+    const uint32_t x = __byte_perm(e, 0, 0x4140);
+    uint32_t v = (x & 0x007f007fu) | 0x43004300u, s = (x & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&s));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// The largest b with pre[b] <= u.
+__device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
+    int lo = 0, hi = B;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= u)
+            lo = mid;
+        else
+            hi = mid;
     }
-    float q[R], o[R] = {};
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-        q[r] = to_f32(static_cast<const Act*>(a.q)[(size_t)b * a.ldq + (size_t)h * D + r * 32 + lane]) * a.scale * kLog2e;
-    float m = -INFINITY, l = 0.0f;
-    for (int t = warp; t < len; t += 4) {
-        const uint32_t pg = a.kv.page_table[(size_t)b * a.kv.max_pages + t / kPageTokens];
-        if (pg >= (uint32_t)a.kv.pool_pages) {
-            if (lane == 0) atomicCAS(a.err, 0, kErrPage);
-            continue;
+    return lo;
+}
+
+struct Item {
+    int b, it, start, units;  // sequence, item of the sequence, first unit, units
+};
+__device__ __forceinline__ Item item_of(const int* pre, int B, int per_seq, int u) {
+    Item x;
+    x.b = find_sequence(pre, B, u);
+    x.units = (pre[x.b + 1] - pre[x.b]) / per_seq;
+    x.it = (u - pre[x.b]) / x.units;
+    x.start = pre[x.b] + x.it * x.units;
+    return x;
+}
+
+// First unit of block c: an equal share of the list, moved to the start of the
+// item it falls into when that item is short.
+__device__ __forceinline__ int cut(const int* pre, int B, int per_seq, int total, int blocks, int c) {
+    const int u = (int)((long long)total * c / blocks);
+    if (c == 0 || u >= total) return u;
+    const Item x = item_of(pre, B, per_seq, u);
+    return x.units <= max(kWholeUnits, total / blocks / 4) ? x.start : u;
+}
+
+// KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item.
+template <int KV, int D, int R>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_attn_kernel(const DecodeAttnArgs a, const Plan plan) {
+    using L = Layout<KV, D>;
+    using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
+    constexpr int kTok = L::kTok, S = L::kStages, kRows = 8 * R;
+    extern __shared__ __align__(128) uint8_t smem[];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int c = blockIdx.x, Hkv = a.kv.n_kv, Hq = a.Hq;
+    const int per_seq = Hkv * plan.tiles;
+    float* stat_m = reinterpret_cast<float*>(smem + L::kStats);  // [warp][16]
+    float* stat_l = stat_m + kWarps * 16;
+    int* stat_buf = reinterpret_cast<int*>(stat_l + kWarps * 16);
+    int* lens = reinterpret_cast<int*>(smem + L::kLens);
+    int* pre = lens + a.B;
+    __shared__ int s_warp[kWarps], s_cut[2];
+    int4* desc = static_cast<int4*>(a.ws);
+    float* slots = reinterpret_cast<float*>(desc + plan.blocks);
+
+    // lengths and units before each sequence
+    {
+        const int per = (a.B + kThreads - 1) / kThreads, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
+        int sum = 0;
+        for (int b = lo; b < hi; ++b) {
+            int n = a.seq_len[b];
+            if (n < 0 || n > a.kv.max_pages * kPageTokens) {
+                if (c == 0) atomicCAS(a.err, 0, kErrSeqLen);
+                n = n < 0 ? 0 : a.kv.max_pages * kPageTokens;
+            }
+            lens[b] = n;
+            pre[b] = sum;
+            sum += (n + kTok - 1) / kTok * per_seq;
         }
-        const size_t row = ((size_t)pg * Hkv + hk) * kPageTokens + t % kPageTokens;
-        float s = 0.0f;
+        int x = sum;
 #pragma unroll
-        for (int r = 0; r < R; ++r) s += q[r] * to_f32(static_cast<const Kv*>(a.kv.k_pool)[row * D + r * 32 + lane]);
-#pragma unroll
-        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-        float vs = 1.0f;
-        if constexpr (sizeof(Kv) == 1) {
-            s *= __half2float(a.kv.k_scale[row]);
-            vs = __half2float(a.kv.v_scale[row]);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
         }
-        const float mn = fmaxf(m, s), alpha = exp2f(m - mn), p = exp2f(s - mn);
-        m = mn;
-        l = l * alpha + p;
-#pragma unroll
-        for (int r = 0; r < R; ++r)
-            o[r] = o[r] * alpha + p * vs * to_f32(static_cast<const Kv*>(a.kv.v_pool)[row * D + r * 32 + lane]);
+        if (lane == 31) s_warp[warp] = x;
+        __syncthreads();
+        int before = x - sum;
+        for (int w = 0; w < warp; ++w) before += s_warp[w];
+        for (int b = lo; b < hi; ++b) pre[b] += before;
+        if (tid == kThreads - 1) pre[a.B] = before + sum;
+        __syncthreads();
     }
-    if (lane == 0) {
-        sm[warp] = m;
-        sl[warp] = l;
+    const int total = pre[a.B];
+    const int blocks = min(plan.blocks, (total + kMinUnits - 1) / kMinUnits);
+
+    // sequences without tokens
+    for (int b = c; b < a.B; b += gridDim.x) {
+        if (lens[b]) continue;
+        for (int i = tid; i < Hq * D; i += kThreads) static_cast<Act*>(a.out)[(size_t)b * Hq * D + i] = (Act)0.0f;
+        if (a.lse)
+            for (int i = tid; i < Hq; i += kThreads) a.lse[(size_t)b * Hq + i] = -INFINITY;
     }
-#pragma unroll
-    for (int r = 0; r < R; ++r) so[warp][r * 32 + lane] = o[r];
+    if (c >= blocks) {
+        if (tid == 0) desc[c] = make_int4(-1, 0, 0, 0);
+        return;
+    }
+    if (tid < 2) s_cut[tid] = cut(pre, a.B, per_seq, total, blocks, c + tid);
     __syncthreads();
-    float M = -INFINITY, L = 0.0f;
-    for (int w = 0; w < 4; ++w) M = fmaxf(M, sm[w]);
-    for (int w = 0; w < 4; ++w) L += M == -INFINITY ? 0.0f : sl[w] * exp2f(sm[w] - M);
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float x = 0.0f;
-        if (M != -INFINITY)
-            for (int w = 0; w < 4; ++w) x += so[w][d] * exp2f(sm[w] - M);
-        static_cast<Act*>(a.out)[((size_t)b * a.Hq + h) * D + d] = (Act)(L > 0.0f ? x / L : 0.0f);
+    const int u0 = s_cut[0], u1 = s_cut[1];
+
+    // ---- this warp's stream of units
+    const int n_w = max(0, (u1 - u0 - warp + kWarps - 1) / kWarps);
+    uint4* ring = reinterpret_cast<uint4*>(smem + L::kRings) + warp * kRing;
+    const uint32_t stage0 = smem_u32(smem + warp * S * L::kStage);
+    auto describe = [&](int j0) {  // the units j0 .. j0 + 31: pages, head, tokens present
+        const int j = j0 + lane;
+        if (j >= n_w) return;
+        const int u = u0 + warp + kWarps * j;
+        const Item x = item_of(pre, a.B, per_seq, u);
+        const int first = (u - x.start) * kTok, left = lens[x.b] - first;
+        const uint32_t* row = a.kv.page_table + (size_t)x.b * a.kv.max_pages + first / kPageTokens;
+        uint4 e = make_uint4(row[0], 0, (uint32_t)(x.it / plan.tiles), left >= 32 ? ~0u : (1u << left) - 1);
+        uint32_t low = kTok == 8 ? 0xffu : 0xffffu;
+        e.w &= kTok == 32 ? ~0u : low;
+        if (e.x >= (uint32_t)a.kv.pool_pages) {
+            atomicCAS(a.err, 0, kErrPage);
+            e.x = 0;
+            e.w &= ~low;
+        }
+        if (kTok == 32 && left > 16) {
+            e.y = row[1];
+            if (e.y >= (uint32_t)a.kv.pool_pages) {
+                atomicCAS(a.err, 0, kErrPage);
+                e.y = 0;
+                e.w &= 0xffffu;
+            }
+        }
+        if (kTok == 8) e.y = first % kPageTokens;  // the page's half
+        ring[j % kRing] = e;
+    };
+    auto issue = [&](int j) {
+        if (j < n_w) {
+            if (j % 32 == 0) {
+                describe(j);
+                __syncwarp();
+            }
+            const uint4 e = ring[j % kRing];
+            const uint32_t st = stage0 + (j % S) * L::kStage;
+            constexpr int kChunks = L::kRow / 16, kPer = 32 / kChunks;  // rows per instruction
+            const int chunk = lane % kChunks;
+            const size_t block0 = ((size_t)e.x * Hkv + e.z) * kPageTokens + (kTok == 8 ? e.y : 0);
+            const size_t block1 = kTok == 32 ? ((size_t)e.y * Hkv + e.z) * kPageTokens : 0;
+#pragma unroll
+            for (int i = 0; i < kTok / kPer; ++i) {
+                const int row = i * kPer + lane / kChunks;
+                const size_t at = ((kTok == 32 && row >= 16 ? block1 + row - 16 : block0 + row) * kChunks + chunk) * 16;
+                const int n = (e.w >> row) & 1 ? 16 : 0;
+                const uint32_t dst = st + row * L::kRow;
+                int kc = chunk, vc = chunk;
+                if (KV == VELO_KV_F16) {
+                    kc ^= row & 7;
+                    vc ^= row & 7;
+                } else if (KV == VELO_KV_INT8) {
+                    kc ^= D == 128 ? (row & 1) << 2 : 0;
+                    vc ^= D == 128 ? row & 6 : (row >> 1) & 3;
+                } else {
+                    kc ^= (row & 1) << 2;
+                }
+                cp_async16(dst + kc * 16, static_cast<const uint8_t*>(a.kv.k_pool) + at, n);
+                cp_async16(dst + L::kHalf + vc * 16, static_cast<const uint8_t*>(a.kv.v_pool) + at, n);
+            }
+            if (KV == VELO_KV_INT8 && lane < 8) {  // scales: K of both pages, V of both pages
+                const int pg = (lane >> 1) & 1, half = lane & 1;
+                const size_t at = (pg ? block1 : block0) + half * 8;
+                const int n = (e.w >> (pg * 16 + half * 8)) & 0xff ? 16 : 0;
+                cp_async16(st + 2 * L::kHalf + lane * 16, (lane < 4 ? a.kv.k_scale : a.kv.v_scale) + at, n);
+            }
+        }
+        cp_async_commit();
+    };
+    for (int j = 0; j < S; ++j) issue(j);
+
+    const float scale = a.scale * kLog2e;
+    int j = 0;
+    int4 open = make_int4(-1, 0, 0, 0);
+    for (int seg = u0; seg < u1;) {
+        const Item x = item_of(pre, a.B, per_seq, seg);
+        const int end = x.start + x.units, seg_end = min(end, u1);
+        const int hk = x.it / plan.tiles, tile = x.it % plan.tiles;
+        const int h0 = hk * plan.group + tile * kRows, nh = min(kRows, plan.group - tile * kRows);
+        const Act* qp = static_cast<const Act*>(a.q) + (size_t)x.b * a.ldq + (size_t)h0 * D;
+
+        // ---- running state: row = 8r + g (f32: rows 2t, 2t + 1 of this lane's token)
+        constexpr int kM = KV == VELO_KV_F32 ? 2 : R;
+        float m[kM], l[kM];
+#pragma unroll
+        for (int r = 0; r < kM; ++r) {
+            m[r] = -INFINITY;
+            l[r] = 0.0f;
+        }
+        constexpr int kN = KV == VELO_KV_F32 ? 1 : D / 8;       // output tiles of 8 dimensions
+        float o[KV == VELO_KV_F32 ? 1 : R][kN][4] = {};
+        constexpr int kO = KV == VELO_KV_F32 ? D / 32 : 1;      // dimensions per lane
+        float of[KV == VELO_KV_F32 ? 8 : 1][kO] = {};
+        uint32_t qa[KV == VELO_KV_F32 ? 1 : D / 16][4];
+        if constexpr (KV == VELO_KV_F32) {
+            float* qs = reinterpret_cast<float*>(smem + L::kQ);
+            for (int i = tid; i < 8 * D; i += kThreads) qs[i] = i / D < nh ? to_f32(qp[i]) : 0.0f;
+            __syncthreads();
+        } else {
+#pragma unroll
+            for (int ks = 0; ks < D / 16; ++ks) {
+                // the dimensions a lane holds of contraction step ks: ldmatrix's own order for
+                // f16, 4 of its 16 consecutive bytes for int8
+                const int d0 = KV == VELO_KV_F16 ? 16 * ks + 2 * t : 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
+                const int d1 = d0 + (KV == VELO_KV_F16 ? 8 : 2);
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int row = 8 * r + g;
+                    const bool live = r < R && row < nh;
+                    qa[ks][r] = live ? *reinterpret_cast<const uint32_t*>(qp + (size_t)row * D + d0) : 0u;
+                    qa[ks][2 + r] = live ? *reinterpret_cast<const uint32_t*>(qp + (size_t)row * D + d1) : 0u;
+                }
+            }
+        }
+        bool pending = false;
+        for (; j < n_w && u0 + warp + kWarps * j < seg_end; ++j) {
+            if (pending) issue(j - 1 + S);
+            cp_async_wait<S - 1>();
+            __syncwarp();
+            const uint32_t st = stage0 + (j % S) * L::kStage;
+            const uint32_t present = ring[j % kRing].w;
+            if constexpr (KV != VELO_KV_F32) {
+                // ---- scores
+                constexpr int kT = kTok / 8;
+                float s[kT][4] = {};
+                if constexpr (KV == VELO_KV_F16) {
+                    const int r = lane & 7, mi = lane >> 3;
+                    const uint32_t kb = st + ((mi >> 1) * 8 + r) * L::kRow;
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        uint32_t kf[4];
+                        ldmatrix_x4(kf, kb + (((2 * ks + (mi & 1)) ^ r) << 4));
+                        mma_f16(s[0], qa[ks], kf[0], kf[1]);
+                        mma_f16(s[1], qa[ks], kf[2], kf[3]);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                        for (int kt = 0; kt < kT; ++kt) {
+                            const int row = kt * 8 + g, ch = (4 * h + t) ^ (D == 128 ? (row & 1) << 2 : 0);
+                            const uint4 w4 = lds128(st + row * L::kRow + ch * 16);
+                            const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u,
+                                                   w4.w ^ 0x80808080u};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                mma_f16(s[kt], qa[4 * h + i], bytes_to_f16<0>(w[i]), bytes_to_f16<1>(w[i]));
+                        }
+                }
+                // ---- softmax of this lane's tokens 8 kt + 2t, + 1 in rows g (and 8 + g)
+                float vs[kT][2];
+                float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                for (int kt = 0; kt < kT; ++kt) {
+                    float f0 = scale, f1 = scale;
+                    const int tok = kt * 8 + 2 * t;
+                    if constexpr (KV == VELO_KV_INT8) {
+                        const float2 ks = lds_half2(st + 2 * L::kHalf + tok * 2);
+                        const float2 vv = lds_half2(st + 2 * L::kHalf + 2 * kTok + tok * 2);
+                        f0 *= ks.x;
+                        f1 *= ks.y;
+                        vs[kt][0] = (present >> tok) & 1 ? vv.x : 0.0f;
+                        vs[kt][1] = (present >> (tok + 1)) & 1 ? vv.y : 0.0f;
+                    }
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        s[kt][2 * r] = (present >> tok) & 1 ? s[kt][2 * r] * f0 : -INFINITY;
+                        s[kt][2 * r + 1] = (present >> (tok + 1)) & 1 ? s[kt][2 * r + 1] * f1 : -INFINITY;
+                        mx[r] = fmaxf(mx[r], fmaxf(s[kt][2 * r], s[kt][2 * r + 1]));
+                    }
+                }
+                float alpha[R], ref[R];
+                bool moved = false;
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                    const float mn = fmaxf(m[r], mx[r]);
+                    ref[r] = mn == -INFINITY ? 0.0f : mn;
+                    alpha[r] = ex2_approx(m[r] - ref[r]);
+                    moved |= mn != m[r];
+                    m[r] = mn;
+                    l[r] *= alpha[r];
+                }
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kN; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) o[r][n][e] *= alpha[r];
+                }
+                // ---- weights as A fragments (rows g: the value, rows 8 + g: its remainder) and P V
+#pragma unroll
+                for (int kk = 0; kk < kT / 2; ++kk) {
+                    uint32_t pa[R][4];
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float p0 = ex2_approx(s[2 * kk + i][2 * r] - ref[r]);
+                            float p1 = ex2_approx(s[2 * kk + i][2 * r + 1] - ref[r]);
+                            l[r] += p0 + p1;
+                            if constexpr (KV == VELO_KV_INT8)
+                                split_bf16(p0 * vs[2 * kk + i][0], p1 * vs[2 * kk + i][1], pa[r][2 * i], pa[r][2 * i + 1]);
+                            else
+                                split_f16(p0, p1, pa[r][2 * i], pa[r][2 * i + 1]);
+                        }
+                    if constexpr (KV == VELO_KV_F16) {
+                        const int r8 = lane & 7, mi = lane >> 3;
+                        const uint32_t vb = st + L::kHalf + ((mi & 1) * 8 + r8) * L::kRow;
+#pragma unroll
+                        for (int n = 0; n < D / 16; ++n) {
+                            uint32_t vf[4];
+                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi >> 1)) ^ r8) << 4));
+#pragma unroll
+                            for (int r = 0; r < R; ++r) {
+                                mma_f16(o[r][2 * n], pa[r], vf[0], vf[1]);
+                                mma_f16(o[r][2 * n + 1], pa[r], vf[2], vf[3]);
+                            }
+                        }
+                    } else {
+                        // dimension n of this lane's column: g * D / 8 + n
+                        uint32_t w[4][D / 32];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int row = kk * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+                            const uint32_t rb = st + L::kHalf + row * L::kRow;
+                            if constexpr (D == 128) {
+                                const uint4 v = lds128(rb + ((g ^ (row & 6)) << 4));
+                                w[i][0] = v.x;
+                                w[i][1] = v.y;
+                                w[i][2] = v.z;
+                                w[i][3] = v.w;
+                            } else {
+                                const uint2 v = lds64(rb + ((((g >> 1) ^ ((row >> 1) & 3)) << 4) | (g & 1) << 3));
+                                w[i][0] = v.x;
+                                w[i][1] = v.y;
+                            }
+                        }
+#pragma unroll
+                        for (int q4 = 0; q4 < D / 32; ++q4) {
+#pragma unroll
+                            for (int r = 0; r < R; ++r) {
+                                mma_bf16(o[r][4 * q4], pa[r], byte_pair_to_bf16<0>(w[0][q4], w[1][q4]),
+                                         byte_pair_to_bf16<0>(w[2][q4], w[3][q4]));
+                                mma_bf16(o[r][4 * q4 + 1], pa[r], byte_pair_to_bf16<1>(w[0][q4], w[1][q4]),
+                                         byte_pair_to_bf16<1>(w[2][q4], w[3][q4]));
+                                mma_bf16(o[r][4 * q4 + 2], pa[r], byte_pair_to_bf16<2>(w[0][q4], w[1][q4]),
+                                         byte_pair_to_bf16<2>(w[2][q4], w[3][q4]));
+                                mma_bf16(o[r][4 * q4 + 3], pa[r], byte_pair_to_bf16<3>(w[0][q4], w[1][q4]),
+                                         byte_pair_to_bf16<3>(w[2][q4], w[3][q4]));
+                            }
+                        }
+                    }
+                }
+            } else {
+                // ---- f32 scores: token g, dimensions 16 i + 4 t .. + 3 of every head
+                const float* qs = reinterpret_cast<const float*>(smem + L::kQ);
+                float* pw = reinterpret_cast<float*>(smem + L::kP) + warp * 72;  // [token][head], then alpha[head]
+                float s[8] = {};
+#pragma unroll 2
+                for (int i = 0; i < D / 16; ++i) {
+                    const uint4 kw = lds128(st + g * L::kRow + (((4 * i + t) ^ ((g & 1) << 2)) << 4));
+                    const float k0 = __uint_as_float(kw.x), k1 = __uint_as_float(kw.y), k2 = __uint_as_float(kw.z),
+                                k3 = __uint_as_float(kw.w);
+#pragma unroll
+                    for (int h = 0; h < 8; ++h) {
+                        const float4 qv = *reinterpret_cast<const float4*>(qs + h * D + 16 * i + 4 * t);
+                        s[h] = fmaf(qv.x, k0, fmaf(qv.y, k1, fmaf(qv.z, k2, fmaf(qv.w, k3, s[h]))));
+                    }
+                }
+                // reduce-scatter over the four lanes of a token: lane t keeps heads 2t, 2t + 1
+                float a4[4], a2[2];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float give = t & 2 ? s[i] : s[4 + i], keep = t & 2 ? s[4 + i] : s[i];
+                    a4[i] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float give = t & 1 ? a4[i] : a4[2 + i], keep = t & 1 ? a4[2 + i] : a4[i];
+                    a2[i] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+                }
+                bool moved = false;
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const float sv = (present >> g) & 1 ? a2[r] * scale : -INFINITY;
+                    float mx = sv;
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                    const float mn = fmaxf(m[r], mx), rf = mn == -INFINITY ? 0.0f : mn;
+                    const float al = ex2_approx(m[r] - rf), p = ex2_approx(sv - rf);
+                    moved |= mn != m[r];
+                    m[r] = mn;
+                    l[r] = l[r] * al + p;
+                    pw[g * 8 + 2 * t + r] = p;
+                    if (g == 0) pw[64 + 2 * t + r] = al;
+                }
+                __syncwarp();
+                if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                    for (int h = 0; h < 8; ++h)
+#pragma unroll
+                        for (int e = 0; e < kO; ++e) of[h][e] *= pw[64 + h];
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float4 pA = *reinterpret_cast<const float4*>(pw + k * 8);
+                    const float4 pB = *reinterpret_cast<const float4*>(pw + k * 8 + 4);
+                    const float p[8] = {pA.x, pA.y, pA.z, pA.w, pB.x, pB.y, pB.z, pB.w};
+                    float v[4];
+                    if constexpr (D == 128) {
+                        const uint4 w = lds128(st + L::kHalf + k * L::kRow + lane * 16);
+                        v[0] = __uint_as_float(w.x);
+                        v[1] = __uint_as_float(w.y);
+                        v[2] = __uint_as_float(w.z);
+                        v[3] = __uint_as_float(w.w);
+                    } else {
+                        const uint2 w = lds64(st + L::kHalf + k * L::kRow + lane * 8);
+                        v[0] = __uint_as_float(w.x);
+                        v[1] = __uint_as_float(w.y);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 8; ++h)
+#pragma unroll
+                        for (int e = 0; e < kO; ++e) of[h][e] = fmaf(p[h], v[e], of[h][e]);
+                }
+            }
+            __syncwarp();  // every lane has read the stage
+            pending = true;
+        }
+
+        // ---- the item's end in this range: the warps' states into one.  A warp's output goes
+        // into the stage it has just read, which is refilled after the join.
+        const uint32_t buf = stage0 + ((j + S - 1) % S) * L::kStage;  // stage of unit j - 1
+        if constexpr (KV == VELO_KV_F32) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
+            if (g == 0) {
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    stat_m[warp * 16 + 2 * t + r] = m[r];
+                    stat_l[warp * 16 + 2 * t + r] = l[r];
+                }
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                if (t == 0) {
+                    stat_m[warp * 16 + 8 * r + g] = m[r];
+                    stat_l[warp * 16 + 8 * r + g] = l[r];
+                }
+            }
+        }
+        if (lane == 0) stat_buf[warp] = (int)(buf - smem_u32(smem));
+        if (pending) {
+            float* dst = reinterpret_cast<float*>(smem + (buf - smem_u32(smem)));
+            if constexpr (KV == VELO_KV_F32) {
+#pragma unroll
+                for (int h = 0; h < 8; ++h)
+#pragma unroll
+                    for (int e = 0; e < kO; ++e) dst[h * D + lane * kO + e] = of[h][e];
+            } else {
+                // fragment order [row][tile][8 columns], tiles XORed with the row against bank conflicts
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int n = 0; n < kN; ++n)
+                        *reinterpret_cast<float2*>(dst + (8 * r + g) * D + ((n ^ g) << 3) + 2 * t) =
+                            make_float2(o[r][n][0] + o[r][n][2], o[r][n][1] + o[r][n][3]);
+            }
+        }
+        __syncthreads();
+        const bool whole = seg == x.start && seg_end == end;
+        const int slot = 2 * c + (seg == x.start ? 1 : 0);
+        float* sp = slots + (size_t)slot * slot_floats(kRows, D);
+        for (int i = tid; i < nh * (D / 2); i += kThreads) {
+            const int row = i / (D / 2), d = i % (D / 2) * 2;
+            float M = -INFINITY, Ls = 0.0f, y0 = 0.0f, y1 = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) M = fmaxf(M, stat_m[w * 16 + row]);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float lw = stat_l[w * 16 + row];
+                if (lw == 0.0f) continue;  // nothing from this warp (its buffer is in flight)
+                const float f = ex2_approx(stat_m[w * 16 + row] - M);
+                const float* src = reinterpret_cast<const float*>(smem + stat_buf[w]) + row * D;
+                float v0, v1;
+                if constexpr (KV == VELO_KV_F32) {
+                    v0 = src[d];
+                    v1 = src[d + 1];
+                } else if constexpr (KV == VELO_KV_F16) {
+                    const float2 v = *reinterpret_cast<const float2*>(src + ((d >> 3 ^ (row & 7)) << 3) + (d & 7));
+                    v0 = v.x;
+                    v1 = v.y;
+                } else {  // dimension = column * D / 8 + tile
+                    const int col = d / (D / 8), n = d % (D / 8);
+                    v0 = src[((n ^ (row & 7)) << 3) + col];
+                    v1 = src[(((n + 1) ^ (row & 7)) << 3) + col];
+                }
+                Ls = fmaf(lw, f, Ls);
+                y0 = fmaf(v0, f, y0);
+                y1 = fmaf(v1, f, y1);
+            }
+            if (whole) {
+                const float inv = Ls == 0.0f ? 0.0f : 1.0f / Ls;
+                Act* op = static_cast<Act*>(a.out) + ((size_t)x.b * Hq + h0 + row) * D + d;
+                if constexpr (KV == VELO_KV_F32)
+                    *reinterpret_cast<float2*>(op) = make_float2(y0 * inv, y1 * inv);
+                else
+                    *reinterpret_cast<__half2*>(op) = __floats2half2_rn(y0 * inv, y1 * inv);
+                if (d == 0 && a.lse)
+                    a.lse[(size_t)x.b * Hq + h0 + row] = Ls == 0.0f ? -INFINITY : (M + log2f(Ls)) * kLn2;
+            } else {
+                *reinterpret_cast<float2*>(sp + 2 * kRows + row * D + d) = make_float2(y0, y1);
+                if (d == 0) *reinterpret_cast<float2*>(sp + 2 * row) = make_float2(M, Ls);
+            }
+        }
+        __syncthreads();
+        if (pending) issue(j - 1 + S);
+        if (!whole && seg == x.start)  // begins here, ends in a later block
+            open = make_int4(x.b, x.it, (int)(((long long)end * blocks - 1) / total), 0);
+        seg = seg_end;
     }
-    if (threadIdx.x == 0 && a.lse) a.lse[(size_t)b * a.Hq + h] = L > 0.0f ? (M + log2f(L)) * kLn2 : -INFINITY;
+    cp_async_wait<0>();
+    if (tid == 0) desc[c] = open;
 }
 
-template <typename Act, typename Kv>
-cudaError_t launch_typed(const DecodeAttnArgs& a, cudaStream_t s) {
-    if (a.kv.head_dim == 64)
-        decode_attn_kernel<Act, Kv, 64><<<a.B * a.Hq, 128, 0, s>>>(a);
-    else
-        decode_attn_kernel<Act, Kv, 128><<<a.B * a.Hq, 128, 0, s>>>(a);
-    return cudaGetLastError();
+// Joins the partial states of the item that block x of the first kernel left
+// open: slot 1 of that block, slot 0 of the following ones.  One block per (open
+// item, query head); a warp adds every fourth state.
+template <typename Act, int D>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnArgs a, const Plan plan, int rows) {
+    __shared__ float wgt[kMaxBlocks], acc[kWarps][D], red[kWarps], red_l[kWarps];
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // the first kernel is complete and visible
+    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int4* desc = static_cast<const int4*>(a.ws);
+    const int4 it = desc[c];
+    if (it.x < 0) return;
+    const int hk = it.y / plan.tiles, tile = it.y % plan.tiles;
+    if (tile * rows + row >= plan.group) return;
+    const int head = hk * plan.group + tile * rows + row;
+    const float* slots = reinterpret_cast<const float*>(desc + plan.blocks);
+    const size_t step = slot_floats(rows, D);
+    const int n = it.z - c + 1;
+    auto state = [&](int i) { return slots + (size_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * step; };
+    float M = -INFINITY;
+    for (int i = tid; i < n; i += kThreads) {
+        const float mi = state(i)[2 * row];
+        wgt[i] = mi;
+        M = fmaxf(M, mi);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red[w]);
+    float Ls = 0.0f;
+    for (int i = tid; i < n; i += kThreads) {
+        const float li = state(i)[2 * row + 1];
+        const float f = li == 0.0f ? 0.0f : ex2_approx(wgt[i] - M);
+        wgt[i] = f;
+        Ls += li * f;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
+    if (lane == 0) red_l[warp] = Ls;
+    __syncthreads();
+    Ls = red_l[0] + red_l[1] + red_l[2] + red_l[3];
+    constexpr int kE = D / 32;
+    float x[kE] = {};
+#pragma unroll 8
+    for (int i = warp; i < n; i += kWarps) {
+        const float f = wgt[i];
+        const float* p = state(i) + 2 * rows + row * D + lane * kE;
+        if (f != 0.0f) {
+#pragma unroll
+            for (int e = 0; e < kE; ++e) x[e] = fmaf(p[e], f, x[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kE; ++e) acc[warp][lane * kE + e] = x[e];
+    __syncthreads();
+    const float inv = Ls == 0.0f ? 0.0f : 1.0f / Ls;
+    for (int d = tid; d < D; d += kThreads)
+        static_cast<Act*>(a.out)[((size_t)it.x * a.Hq + head) * D + d] =
+            (Act)((acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) * inv);
+    if (tid == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = Ls == 0.0f ? -INFINITY : (M + log2f(Ls)) * kLn2;
 }
+
+template <int KV, int D, int R>
+cudaError_t launch_typed(const DecodeAttnArgs& a, int blocks, cudaStream_t s) {
+    using L = Layout<KV, D>;
+    static SmemAttr attr;
+    const int smem = L::kLens + (2 * a.B + 1) * 4;
+    cudaError_t e = ensure_smem(attr, decode_attn_kernel<KV, D, R>, smem);
+    if (e != cudaSuccess) return e;
+    Plan p;
+    p.blocks = blocks;
+    p.group = a.Hq / a.kv.n_kv;
+    p.tiles = (p.group + 8 * R - 1) / (8 * R);
+    decode_attn_kernel<KV, D, R><<<blocks, kThreads, smem, s>>>(a, p);
+    e = cudaGetLastError();
+    // no sequence of this table can reach an item that is cut
+    if (e != cudaSuccess || (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok <= kWholeUnits) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(blocks, std::min(8 * R, p.group));
+    cfg.blockDim = kThreads;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
+    return cudaLaunchKernelEx(&cfg, decode_join_kernel<Act, D>, a, p, 8 * R);
+}
+
+template <int KV, int R>
+cudaError_t launch_rows(const DecodeAttnArgs& a, int blocks, cudaStream_t s) {
+    return a.kv.head_dim == 64 ? launch_typed<KV, 64, R>(a, blocks, s) : launch_typed<KV, 128, R>(a, blocks, s);
+}
+
+int grid_blocks(int sm_count) { return std::min(kBlocksPerSm * sm_count, kMaxBlocks); }
+// tiles of 8 query heads per item: f32 items hold 8 heads, the others up to 16
+int row_tiles(int group, int kv_dtype) { return kv_dtype != VELO_KV_F32 && group > 8 ? 2 : 1; }
 
 }  // namespace
 
-size_t decode_attn_workspace(int, int, int, int) { return 16; }
+size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
+    const size_t blocks = grid_blocks(sm_count);
+    return blocks * sizeof(int4) + 2 * blocks * slot_floats(8 * row_tiles(Hq / Hkv, VELO_KV_F16), D) * sizeof(float);
+}
 
-cudaError_t launch_decode_attention(const DecodeAttnArgs& a, int, cudaStream_t s) {
-    if (a.kv.kv_dtype == VELO_KV_F32) return launch_typed<float, float>(a, s);
-    if (a.kv.kv_dtype == VELO_KV_INT8) return launch_typed<__half, int8_t>(a, s);
-    return launch_typed<__half, __half>(a, s);
+cudaError_t launch_decode_attention(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
+    const int blocks = grid_blocks(sm_count), R = row_tiles(a.Hq / a.kv.n_kv, a.kv.kv_dtype);
+    if (a.kv.kv_dtype == VELO_KV_F32) return launch_rows<VELO_KV_F32, 1>(a, blocks, s);
+    if (a.kv.kv_dtype == VELO_KV_INT8)
+        return R == 2 ? launch_rows<VELO_KV_INT8, 2>(a, blocks, s) : launch_rows<VELO_KV_INT8, 1>(a, blocks, s);
+    return R == 2 ? launch_rows<VELO_KV_F16, 2>(a, blocks, s) : launch_rows<VELO_KV_F16, 1>(a, blocks, s);
 }
 
 }  // namespace velo
