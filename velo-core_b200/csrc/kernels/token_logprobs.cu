@@ -1,7 +1,7 @@
 // token_logprobs.cu -- log probability of given tokens, entropy and the best
 // alternatives of each logits row (velo_cuda_token_logprobs).
 //
-// With m the row's maximum, k = log2(e) / T, u = (x - m) k: Z = sum 2^u, Y = sum u 2^u,
+// With m close to the row's maximum, k = log2(e) / T, u = (x - m) k: Z = sum 2^u, Y = sum u 2^u,
 // log probability = (x[token] - m) / T - ln Z, entropy = ln Z - ln 2 Y / Z.
 // Each logit is read once from HBM, which bounds the kernel.
 //
@@ -21,6 +21,7 @@
 // With a cluster each block sends its sums and its own n best to the first one's
 // shared memory, which ranks them.
 #include <algorithm>
+#include <type_traits>
 
 #include "common/elem.cuh"
 #include "common/sm100.cuh"
@@ -39,20 +40,22 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kErrToken = 0x6221;
 constexpr int kVecs = 4;                              // 16-byte vectors per thread and tile
 constexpr int kTileVecs = kVecs * kThreads;           // 16 KB
-constexpr int kStages = 3;
+constexpr int kStages = 2;
+constexpr int kBlocksPerSm = 4;
 constexpr int kSlots = 16;                            // pieces of the row with their own maxima
 constexpr int kList = 512;                            // candidates before the bound is raised
 constexpr int kMaxCluster = 8;
 constexpr float kLn2 = 0.693147180559945309f;
 
-// Dynamic shared memory.  After the stream the ring holds the selection's lists.
+// Dynamic shared memory: the ring (after the stream: the candidates and the pieces
+// to read again), the pieces' maxima, the inbox.
 constexpr int kRingBytes = kStages * kTileVecs * 16;
+constexpr int kWorkOfs = (kList + kMaxTop) * 8;
 constexpr int kSlotOfs = kRingBytes;
-constexpr int kInboxOfs = kSlotOfs + kSlots * kThreads * 4;
-constexpr int kInboxStride = kMaxTop * 8 + 16;        // sorted keys, then m, Z, Y, count
-constexpr int kSmemOne = kInboxOfs + kInboxStride;
+constexpr int kSmemOne = kSlotOfs + kSlots * kThreads * 4;
+constexpr int kInboxOfs = kSmemOne;
+constexpr int kInboxStride = kMaxTop * 8 + 16;  // sorted keys, then m, Z, Y, count
 constexpr int kSmemCluster = kInboxOfs + kMaxCluster * kInboxStride;
-constexpr int kWorkOfs = (kList + kMaxTop) * 8;       // u16 pieces to read again
 static_assert(kWorkOfs + kSlots * kThreads * 2 <= kRingBytes, "lists fit the ring");
 static_assert(kMaxCluster * kMaxTop <= kList + kMaxTop, "a cluster's lists fit the list");
 
@@ -105,12 +108,12 @@ __device__ __forceinline__ void unpack(const __nv_bfloat16*, uint4 v, float* x) 
     }
 }
 
-// Running sums: m is the largest logit, Z and Y belong to u = (x - m) k.  (x - m
+// Running sums: m is a logit near the largest, Z and Y belong to u = (x - m) k.  (x - m
 // rather than one fma: a row masked with the type's lowest value must not overflow.)
 struct Sums {
     float m, z, y;
 };
-// What x is measured from while the largest logit is m.
+// What x is measured from.
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.0f : m; }
 __device__ __forceinline__ Sums join(Sums a, Sums b, float k) {
     Sums r;
@@ -123,6 +126,17 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float k) {
     // (a factor of 0 must not meet an infinite difference)
     r.y = fa * a.y + fb * b.y + (fa > 0.0f ? fa * da * a.z : 0.0f) + (fb > 0.0f ? fb * db * b.z : 0.0f);
     return r;
+}
+// Sums over the first `lanes` lanes of a warp (a power of two), in lane 0.
+__device__ __forceinline__ Sums warp_join(Sums s, float k, int lanes) {
+    float m = s.m;
+    for (int o = lanes / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    s = join(s, Sums{m, 0.0f, 0.0f}, k);
+    for (int o = lanes / 2; o; o >>= 1) {
+        s.z += __shfl_xor_sync(0xffffffffu, s.z, o);
+        s.y += __shfl_xor_sync(0xffffffffu, s.y, o);
+    }
+    return s;
 }
 __device__ __forceinline__ void raise(Sums& s, float m, float k) {
     if (m > s.m) s = join(s, Sums{m, 0.0f, 0.0f}, k);
@@ -160,8 +174,19 @@ __device__ __forceinline__ void rank_list(const unsigned long long* list, int c,
     }
 }
 
+// This block's part of a row: elements [lo, hi), of them nv whole 16-byte vectors
+// from `body` on (element `first`); the row's ragged ends belong to its first
+// and last part.
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const TokenLogprobsArgs a, int cluster) {
+struct Part {
+    const T* row;
+    const T* body;
+    int first, nv, lo, hi;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(const TokenLogprobsArgs a,
+                                                                              int log_cluster) {
     constexpr int kN = Vec<T>::n;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums s_part[kWarps];
@@ -169,202 +194,235 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Token
     __shared__ int s_count, s_work, s_warp[kWarps];
     __shared__ unsigned long long s_raise;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int r = blockIdx.x / cluster, part = blockIdx.x % cluster;
+    const int cluster = 1 << log_cluster, part = blockIdx.x & (cluster - 1), r = blockIdx.x >> log_cluster;
     if (cluster > 1) cluster_arrive();  // the first block's inbox may be written once all have started
-    const T* row = static_cast<const T*>(a.logits) + (size_t)r * a.ldl;
     const float k = a.inv_t * kLog2e;
-    float tok_x = 0.0f;
-    uint32_t tok = 0;
-    if (a.logprob && part == 0 && tid == 0) {
-        tok = a.tokens[r];
-        if (tok < (uint32_t)a.V) tok_x = to_f32(row[tok]);
-    }
-
-    // elements [lo, hi) of this block: aligned vectors, and the row's ragged ends
-    const int head = min(a.V, (int)((16 - (uintptr_t)row % 16) % 16 / sizeof(T)));
-    const int nv_row = (a.V - head) / kN;
-    const int v0 = (int)((long long)nv_row * part / cluster), v1 = (int)((long long)nv_row * (part + 1) / cluster);
-    const int lo = part == 0 ? 0 : head + v0 * kN, hi = part == cluster - 1 ? a.V : head + v1 * kN;
-    const int nv = v1 - v0, tiles = (nv + kTileVecs - 1) / kTileVecs, per_slot = (tiles + kSlots - 1) / kSlots;
-    const T* body = row + head + (size_t)v0 * kN;
     float* slot_max = reinterpret_cast<float*>(smem + kSlotOfs);
+    unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
+    uint16_t* work = reinterpret_cast<uint16_t*>(smem + kWorkOfs);
 
-    auto issue = [&](int tile) {
-        if (tile < tiles) {
-            const uint32_t st = smem_u32(smem) + (tile % kStages) * kTileVecs * 16 + tid * 16;
+    Part<T> p;
+    {
+        p.row = static_cast<const T*>(a.logits) + (size_t)r * a.ldl;
+        const int head = min(a.V, (int)((16 - (uintptr_t)p.row % 16) % 16 / sizeof(T)));
+        const int nv_row = (a.V - head) / kN;  // < 2^22
+        const int v0 = (nv_row * part) >> log_cluster, v1 = (nv_row * (part + 1)) >> log_cluster;
+        p.first = head + v0 * kN;
+        p.nv = v1 - v0;
+        p.lo = part == 0 ? 0 : p.first;
+        p.hi = part == cluster - 1 ? a.V : head + v1 * kN;
+        p.body = p.row + p.first;
+    }
+    const int nv = p.nv, whole_tiles = nv / kTileVecs, tiles = (nv + kTileVecs - 1) / kTileVecs;
+    const int per_slot = (tiles + kSlots - 1) / kSlots;
+    const uint32_t ring = smem_u32(smem) + tid * 16;
+    auto issue = [&](int tile, uint32_t stage) {
+        const uint32_t st = ring + stage;
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(p.body) + ((size_t)tile * kTileVecs + tid) * 16;
+        const int left = p.nv - tile * kTileVecs;
+        if (left >= kTileVecs) {
 #pragma unroll
-            for (int q = 0; q < kVecs; ++q) {
-                const int v = tile * kTileVecs + q * kThreads + tid;
-                const int n = v < nv ? 16 : 0;
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(st + q * kThreads * 16),
-                             "l"(body + (size_t)(n ? v : 0) * kN), "r"(n)
+            for (int q = 0; q < kVecs; ++q)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(st + q * kThreads * 16),
+                             "l"(from + q * kThreads * 16)
                              : "memory");
-            }
+        } else if (left > 0) {
+#pragma unroll
+            for (int q = 0; q < kVecs; ++q)
+                if (q * kThreads + tid < left)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(st + q * kThreads * 16),
+                                 "l"(from + q * kThreads * 16)
+                                 : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    for (int i = 0; i < kStages; ++i) issue(i);
+    for (int i = 0; i < kStages; ++i) issue(i, i * kTileVecs * 16);
 
-    Sums s{-INFINITY, 0.0f, 0.0f};
-    // the ragged ends, one element per thread: index, or -1
+    if (tid == 0) s_count = s_work = 0;
+    uint32_t tok = 0;
+    if (a.logprob && part == 0 && tid == 0) tok = a.tokens[r];
+    // the row's ragged ends, one element per thread: its index, or -1
     int ragged = -1;
-    if (tid < head && part == 0) ragged = tid;
-    const int tail0 = head + nv_row * kN;
-    if (part == cluster - 1 && tid >= 32 && tid - 32 < a.V - tail0) ragged = tail0 + tid - 32;
+    if (part == 0 && tid < p.first) ragged = tid;
+    if (tid >= 32 && p.first + nv * kN + tid - 32 < p.hi) ragged = p.first + nv * kN + tid - 32;
+
+    // ---- this thread's share: sums, largest element, the pieces' maxima
+    Sums s{-INFINITY, 0.0f, 0.0f};
     if (ragged >= 0) {
-        const float x = to_f32(row[ragged]);
+        const float x = to_f32(p.row[ragged]);
         raise(s, x, k);
         float2 z = f2(0.0f), y = f2(0.0f);
         add_two(z, y, x, -INFINITY, f2(-base_of(s.m)), f2(k));
         s.z += z.x;
         s.y += y.x;
     }
-
-    float piece = -INFINITY;
-    for (int tile = 0; tile < tiles; ++tile) {
+    // m is raised only when 2^u could pass 2^8, so that few tiles rescale the sums
+    const float slack = 8.0f / k;
+    float best = s.m, piece = -INFINITY, limit = s.m + slack;
+    int left = per_slot, slot = tid;  // tiles left of the piece, its place in slot_max
+    uint32_t stage = 0;
+    auto consume = [&](int tile, auto whole) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
-        const uint8_t* st = smem + (tile % kStages) * kTileVecs * 16 + tid * 16;
-        const bool full = (tile + 1) * kTileVecs <= nv;
+        const uint8_t* st = smem + stage + tid * 16;
         float x[kVecs * kN];
 #pragma unroll
-        for (int q = 0; q < kVecs; ++q) unpack(row, *reinterpret_cast<const uint4*>(st + q * kThreads * 16), x + q * kN);
-        if (!full) {
+        for (int q = 0; q < kVecs; ++q)
+            unpack(p.row, *reinterpret_cast<const uint4*>(st + q * kThreads * 16), x + q * kN);
+        if constexpr (!decltype(whole)::value) {
 #pragma unroll
             for (int q = 0; q < kVecs; ++q)
                 if (tile * kTileVecs + q * kThreads + tid >= nv) {
 #pragma unroll
                     for (int e = 0; e < kN; ++e) x[q * kN + e] = -INFINITY;
                 }
+        } else {
+            issue(tile + kStages, stage);  // the stage's values are in registers
+            stage = stage == (kStages - 1) * kTileVecs * 16 ? 0 : stage + kTileVecs * 16;
         }
-        issue(tile + kStages);  // the stage's values are in registers
-        float m = x[0];
+        // the maximum three at a time, in two chains
+        float m = x[0], m1 = x[1];
 #pragma unroll
-        for (int i = 1; i < kVecs * kN; ++i) m = fmaxf(m, x[i]);
-        piece = fmaxf(piece, m);
-        raise(s, m, k);
+        for (int i = 2; i + 3 < kVecs * kN; i += 4) {
+            m = max3(m, x[i], x[i + 1]);
+            m1 = max3(m1, x[i + 2], x[i + 3]);
+        }
+        m = max3(max3(m, m1, piece), x[kVecs * kN - 2], x[kVecs * kN - 1]);
+        piece = m;
+        if (__any_sync(0xffffffffu, m > limit)) {
+            raise(s, m, k);
+            limit = s.m + slack;
+        }
         const float2 minus_m = f2(-base_of(s.m));
         float2 z = f2(0.0f), y = f2(0.0f);
 #pragma unroll
         for (int i = 0; i < kVecs * kN; i += 2) add_two(z, y, x[i], x[i + 1], minus_m, f2(k));
         s.z += z.x + z.y;
         s.y += y.x + y.y;
-        if ((tile + 1) % per_slot == 0 || tile + 1 == tiles) {
-            slot_max[tile / per_slot * kThreads + tid] = piece;
+        if (--left == 0 || tile + 1 == tiles) {
+            slot_max[slot] = piece;
+            best = fmaxf(best, piece);
             piece = -INFINITY;
+            left = per_slot;
+            slot += kThreads;
         }
-    }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    };
+    for (int tile = 0; tile < whole_tiles; ++tile) consume(tile, std::true_type{});
+    if (whole_tiles < tiles) consume(whole_tiles, std::false_type{});
+    float tok_x = 0.0f;
+    if (tok < (uint32_t)a.V && a.logprob && part == 0 && tid == 0) tok_x = to_f32(p.row[tok]);
 
-    // ---- the block's sums, and each warp's bound for the selection
-    const uint32_t top_key = order_key(s.m);
-    Sums w = s;
+    // ---- the block's n best as a list, its sums in s_part
+    const int want = min(a.n_top, p.hi - p.lo);
+    // adds every element with key > bound (or >= if ties) to the list
+    auto gather = [&](uint32_t bound, bool ties) {
+        const float floor = bound ? key_value(bound) : -INFINITY;
+        const bool ge = ties || bound == 0, nan = ties && bound == 0;
+        auto reaches = [&](float x) { return ge ? x >= floor || (nan && x != x) : x > floor; };
+        auto offer = [&](float x, int i) {
+            if (!reaches(x)) return;
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kList) list[at] = full_key(order_key(x), i);
+        };
+        if (nan || reaches(best)) {
+            for (int i = 0; i * per_slot < tiles; ++i)
+                if (nan || reaches(slot_max[i * kThreads + tid]))
+                    work[atomicAdd(&s_work, 1)] = (uint16_t)(i * kThreads + tid);
+        }
+        if (ragged >= 0) offer(to_f32(p.row[ragged]), ragged);
+        __syncthreads();
+        // eight lanes read a piece's vectors
+        const int n = s_work;
+        for (int i = tid >> 3; i < n; i += kThreads / 8) {
+            const int at = work[i], first = at / kThreads * per_slot;
+            for (int j = tid & 7; j < per_slot * kVecs; j += 8) {
+                const int v = (first + j / kVecs) * kTileVecs + (j % kVecs) * kThreads + at % kThreads;
+                if (v >= nv) continue;
+                float x[kN];
+                unpack(p.row, __ldg(reinterpret_cast<const uint4*>(p.body + (size_t)v * kN)), x);
 #pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const Sums x{__shfl_xor_sync(0xffffffffu, w.m, o), __shfl_xor_sync(0xffffffffu, w.z, o),
-                     __shfl_xor_sync(0xffffffffu, w.y, o)};
-        // the same order on both sides of the exchange
-        w = lane & o ? join(x, w, k) : join(w, x, k);
-    }
-    const int full_warps = min(kWarps, nv / 32);  // warps whose every lane has data
-    const int each = full_warps ? (a.n_top + full_warps - 1) / full_warps : 0;
+                for (int e = 0; e < kN; ++e) offer(x[e], p.first + v * kN + e);
+            }
+        }
+    };
+    auto post_sums = [&] {
+        s = warp_join(s, k, 32);
+        if (lane == 0) s_part[warp] = s;
+    };
+    uint32_t bound = 0;
     if (a.n_top) {
-        uint32_t key = top_key, bound = 0;
+        const int full_warps = min(kWarps, nv / 32);  // warps whose every lane has data
+        const int each = full_warps ? (a.n_top + full_warps - 1) / full_warps : 0;
+        uint32_t key = order_key(best);
         for (int i = 0; i < each; ++i) {
             bound = __reduce_max_sync(0xffffffffu, key);
             const uint32_t who = __ballot_sync(0xffffffffu, key == bound);
             if (lane == __ffs(who) - 1) key = 0;
         }
         if (lane == 0) s_bound[warp] = bound;
-    }
-    if (lane == 0) s_part[warp] = w;
-    __syncthreads();
-    s = s_part[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) s = join(s, s_part[i], k);
-
-    // ---- the block's n best, sorted, into its inbox
-    unsigned long long* list = reinterpret_cast<unsigned long long*>(smem);
-    uint16_t* work = reinterpret_cast<uint16_t*>(smem + kWorkOfs);
-    unsigned long long* mine = reinterpret_cast<unsigned long long*>(smem + kInboxOfs);
-    const int want = min(a.n_top, hi - lo);
-    if (a.n_top) {
-        // every element with key > bound (or >= if ties) into the list; the number found
-        auto collect = [&](uint32_t bound, bool ties) {
-            __syncthreads();
-            if (tid == 0) s_count = s_work = 0;
-            __syncthreads();
-            for (int i = 0; i * per_slot < tiles; ++i) {
-                const uint32_t mk = order_key(slot_max[i * kThreads + tid]);
-                if (mk > bound || (ties && mk == bound)) work[atomicAdd(&s_work, 1)] = (uint16_t)(i * kThreads + tid);
-            }
-            auto offer = [&](float x, int i) {
-                const uint32_t kx = order_key(x);
-                if (kx > bound || (ties && kx == bound)) {
-                    const int at = atomicAdd(&s_count, 1);
-                    if (at < kList) list[at] = full_key(kx, i);
-                }
-            };
-            if (ragged >= 0) offer(to_f32(row[ragged]), ragged);
-            __syncthreads();
-            const int per = per_slot * kVecs, n = s_work * per;
-            for (int i = tid; i < n; i += kThreads) {
-                const int p = work[i / per], j = i % per;
-                const int v = ((p / kThreads) * per_slot + j / kVecs) * kTileVecs + (j % kVecs) * kThreads + p % kThreads;
-                if (v >= nv || (p / kThreads) * per_slot + j / kVecs >= tiles) continue;
-                float x[kN];
-                unpack(row, __ldg(reinterpret_cast<const uint4*>(body + (size_t)v * kN)), x);
-#pragma unroll
-                for (int e = 0; e < kN; ++e) offer(x[e], head + (v0 + v) * kN + e);
-            }
-            __syncthreads();
-            return s_count;
-        };
-        // appends the first `need` elements equal to the bound, in index order
-        auto add_ties = [&](uint32_t bound, int c, int need) {
-            int seen = 0;
-            for (int base = lo; base < hi && seen < need; base += kThreads) {
-                const int i = base + tid;
-                const bool tie = i < hi && order_key(to_f32(row[i])) == bound;
-                const uint32_t bal = __ballot_sync(0xffffffffu, tie);
-                if (lane == 0) s_warp[warp] = __popc(bal);
-                __syncthreads();
-                int before = seen + __popc(bal & ((1u << lane) - 1));
-#pragma unroll
-                for (int j = 0; j < kWarps; ++j) {
-                    if (j < warp) before += s_warp[j];
-                    seen += s_warp[j];
-                }
-                if (tie && before < need) list[c + before] = full_key(bound, i);
-                __syncthreads();
-            }
-            return c + min(seen, need);
-        };
-        uint32_t bound = full_warps ? 0xffffffffu : 0u;
+        __syncthreads();
+        bound = full_warps ? 0xffffffffu : 0u;
         for (int i = 0; i < full_warps; ++i) bound = min(bound, s_bound[i]);
-        int c = collect(bound, true);
-        if (c > kList) {
-            while ((c = collect(bound, false)) > kList) {
-                // a higher bound: the want-th best of those listed
+    } else {
+        __syncthreads();
+    }
+    int c = 0;
+    if (a.n_top) {
+        bool ties = true;
+        for (;;) {
+            gather(bound, ties);
+            if (ties) post_sums();
+            __syncthreads();
+            c = s_count;
+            // complete: everything from the bound on, or everything above it
+            if (c <= kList && (!ties || c >= want)) break;
+            if (c > kList && !ties) {  // a higher bound: the want-th best of those listed
                 rank_list(list, kList, [&](int rank, unsigned long long key) {
                     if (rank == want - 1) s_raise = key;
                 });
                 __syncthreads();
                 bound = (uint32_t)(s_raise >> 32);
+            } else if (c < want) {  // NaN entries among the best: below everything else
+                bound = 0;
             }
-            if (c < want) c = add_ties(bound, c, want - c);
-        } else if (c < want) {  // NaN entries among the best: below everything else, in index order
-            c = collect(0u, false);
-            if (c < want) c = add_ties(0u, c, want - c);
+            ties = false;
+            __syncthreads();
+            if (tid == 0) s_count = s_work = 0;
+            __syncthreads();
         }
+        // the first elements equal to the bound, in index order
+        const int need = want - c;
+        int seen = 0;
+        for (int base = p.lo; base < p.hi && seen < need; base += kThreads) {
+            const int i = base + tid;
+            const bool tie = i < p.hi && order_key(to_f32(p.row[i])) == bound;
+            const uint32_t bal = __ballot_sync(0xffffffffu, tie);
+            if (lane == 0) s_warp[warp] = __popc(bal);
+            __syncthreads();
+            int before = seen + __popc(bal & ((1u << lane) - 1));
+            for (int j = 0; j < kWarps; ++j) {
+                if (j < warp) before += s_warp[j];
+                seen += s_warp[j];
+            }
+            if (tie && before < need) list[c + before] = full_key(bound, i);
+            __syncthreads();
+        }
+        if (need > 0) c += min(seen, need);
+    } else {
+        post_sums();
         __syncthreads();
+    }
+    s = warp_join(s_part[lane % kWarps], k, kWarps);
+    s.m = __shfl_sync(0xffffffffu, s.m, 0);
+    s.z = __shfl_sync(0xffffffffu, s.z, 0);
+    s.y = __shfl_sync(0xffffffffu, s.y, 0);
+
+    // ---- over the cluster (which has one row)
+    if (cluster > 1) {
+        unsigned long long* mine = reinterpret_cast<unsigned long long*>(smem + kInboxOfs);
         rank_list(list, c, [&](int rank, unsigned long long key) {
             if (rank < want) mine[rank] = key;
         });
         __syncthreads();
-    }
-
-    // ---- over the cluster
-    if (cluster > 1) {
         cluster_wait();  // all blocks have started
         if (part != 0) {
             const uint32_t box = map_to_first(smem_u32(smem + kInboxOfs + part * kInboxStride));
@@ -378,20 +436,16 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Token
         cluster_arrive();  // release
         cluster_wait();    // acquire (the others only stay until the first has their data)
         if (part != 0) return;
-        int c = want;
+        c = want;
         for (int i = tid; i < want; i += kThreads) list[i] = mine[i];
-        for (int p = 1; p < cluster; ++p) {
-            const uint8_t* box = smem + kInboxOfs + p * kInboxStride;
+        for (int q = 1; q < cluster; ++q) {
+            const uint8_t* box = smem + kInboxOfs + q * kInboxStride;
             const float* f = reinterpret_cast<const float*>(box + kMaxTop * 8);
             s = join(s, Sums{f[0], f[1], f[2]}, k);
             const int n = __float_as_int(f[3]);
             for (int i = tid; i < n; i += kThreads) list[c + i] = reinterpret_cast<const unsigned long long*>(box)[i];
             c += n;
         }
-        __syncthreads();
-        rank_list(list, c, [&](int rank, unsigned long long key) {
-            if (rank < a.n_top) mine[rank] = key;
-        });
         __syncthreads();
     }
 
@@ -409,30 +463,31 @@ __global__ void __launch_bounds__(kThreads, 3) token_logprobs_kernel(const Token
         }
         if (a.entropy) a.entropy[r] = s.z == 0.0f ? 0.0f : log_z - kLn2 * (s.y / s.z);
     }
-    for (int i = tid; i < a.n_top; i += kThreads) {
-        const unsigned long long key = mine[i];
-        a.top_tokens[(size_t)r * a.n_top + i] = ~(uint32_t)key;
-        a.top_logprobs[(size_t)r * a.n_top + i] = lp(key_value((uint32_t)(key >> 32)));
-    }
+    if (a.n_top)
+        rank_list(list, c, [&](int rank, unsigned long long key) {
+            if (rank >= a.n_top) return;
+            a.top_tokens[(size_t)r * a.n_top + rank] = ~(uint32_t)key;
+            a.top_logprobs[(size_t)r * a.n_top + rank] = lp(key_value((uint32_t)(key >> 32)));
+        });
 }
 
 // Blocks per row: enough for two blocks per SM, as long as each keeps a tile's worth.
-int cluster_of(const TokenLogprobsArgs& a, int sm_count) {
+int log_cluster_of(const TokenLogprobsArgs& a, int sm_count) {
     const int per_tile = kTileVecs * (a.dtype == VELO_ELEM_F32 ? 4 : 8);
-    int c = 1;
-    while (c < kMaxCluster && (long long)a.M * c < 2LL * sm_count && a.V / (2 * c) >= per_tile) c *= 2;
+    int c = 0;
+    while (1 << c < kMaxCluster && ((long long)a.M << c) < 2LL * sm_count && a.V >> (c + 1) >= per_tile) ++c;
     return c;
 }
 
 template <typename T>
 cudaError_t launch_typed(const TokenLogprobsArgs& a, int sm_count, cudaStream_t s) {
     static SmemAttr attr;
-    const int cluster = cluster_of(a, sm_count);
+    const int log_cluster = log_cluster_of(a, sm_count), cluster = 1 << log_cluster;
     const int smem = cluster > 1 ? kSmemCluster : kSmemOne;
     cudaError_t e = ensure_smem(attr, token_logprobs_kernel<T>, kSmemCluster);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = (unsigned)a.M * cluster;
+    cfg.gridDim = (unsigned)a.M << log_cluster;
     cfg.blockDim = kThreads;
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -442,7 +497,7 @@ cudaError_t launch_typed(const TokenLogprobsArgs& a, int sm_count, cudaStream_t 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, cluster);
+    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, log_cluster);
 }
 
 }  // namespace
