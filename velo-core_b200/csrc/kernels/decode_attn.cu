@@ -157,8 +157,7 @@ __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
 // bits is 128 + them, 0x4300 | sign bit is 128 or 256.
 template <int b>
 __device__ __forceinline__ uint32_t byte_pair_to_bf16(uint32_t w0, uint32_t w1) {
-    const uint32_t e = __byte_perm(w0, w1, b | (4 + b) << 4);  // bytes: w0.b, w1.b, w0.0, w0.0
-    const uint32_t x = __byte_perm(e, 0, 0x4140);
+    const uint32_t x = __byte_perm(w0, w1, b | b << 4 | (4 + b) << 8 | (4 + b) << 12);  // odd bytes are masked out
     uint32_t v = (x & 0x007f007fu) | 0x43004300u, s = (x & 0x00800080u) | 0x43004300u;
     const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&s));
     return *reinterpret_cast<const uint32_t*>(&r);
@@ -294,6 +293,19 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_attn_kernel(con
         if (kTok == 8) e.y = first % kPageTokens;  // the page's half
         ring[j % kRing] = e;
     };
+    // An instruction copies 512 bytes: 32 chunks of kPer rows.  Chunk c of row r lies at
+    // c ^ swizzle(r) of its row; the swizzles split into a part of the instruction
+    // and one of the lane.
+    constexpr int kChunks = L::kRow / 16, kPer = 32 / kChunks, kIts = kTok / kPer;
+    auto k_swizzle = [](int row) {
+        return KV == VELO_KV_F16 ? row & 7 : KV == VELO_KV_INT8 && D == 64 ? 0 : (row & 1) << 2;
+    };
+    auto v_swizzle = [](int row) {
+        return KV == VELO_KV_F16 ? row & 7 : KV == VELO_KV_F32 ? 0 : D == 128 ? row & 6 : (row >> 1) & 3;
+    };
+    const uint32_t k_dst = lane / kChunks * L::kRow + (((lane % kChunks) ^ k_swizzle(lane / kChunks)) << 4);
+    const uint32_t v_dst = lane / kChunks * L::kRow + (((lane % kChunks) ^ v_swizzle(lane / kChunks)) << 4);
+    constexpr uint32_t kFull = kTok == 32 ? ~0u : (1u << kTok) - 1;
     auto issue = [&](int j) {
         if (j < n_w) {
             if (j % 32 == 0) {
@@ -302,32 +314,25 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_attn_kernel(con
             }
             const uint4 e = ring[j % kRing];
             const uint32_t st = stage0 + (j % S) * L::kStage;
-            constexpr int kChunks = L::kRow / 16, kPer = 32 / kChunks;  // rows per instruction
-            const int chunk = lane % kChunks;
             const size_t block0 = ((size_t)e.x * Hkv + e.z) * kPageTokens + (kTok == 8 ? e.y : 0);
-            const size_t block1 = kTok == 32 ? ((size_t)e.y * Hkv + e.z) * kPageTokens : 0;
+            const size_t block1 = kTok == 32 ? ((size_t)e.y * Hkv + e.z) * kPageTokens - 16 : block0;
+            const uint8_t* k0 = static_cast<const uint8_t*>(a.kv.k_pool) + block0 * L::kRow + lane * 16;
+            const uint8_t* v0 = static_cast<const uint8_t*>(a.kv.v_pool) + block0 * L::kRow + lane * 16;
+            const uint8_t* k1 = static_cast<const uint8_t*>(a.kv.k_pool) + block1 * L::kRow + lane * 16;
+            const uint8_t* v1 = static_cast<const uint8_t*>(a.kv.v_pool) + block1 * L::kRow + lane * 16;
+            const bool full = e.w == kFull;
 #pragma unroll
-            for (int i = 0; i < kTok / kPer; ++i) {
-                const int row = i * kPer + lane / kChunks;
-                const size_t at = ((kTok == 32 && row >= 16 ? block1 + row - 16 : block0 + row) * kChunks + chunk) * 16;
-                const int n = (e.w >> row) & 1 ? 16 : 0;
-                const uint32_t dst = st + row * L::kRow;
-                int kc = chunk, vc = chunk;
-                if (KV == VELO_KV_F16) {
-                    kc ^= row & 7;
-                    vc ^= row & 7;
-                } else if (KV == VELO_KV_INT8) {
-                    kc ^= D == 128 ? (row & 1) << 2 : 0;
-                    vc ^= D == 128 ? row & 6 : (row >> 1) & 3;
-                } else {
-                    kc ^= (row & 1) << 2;
-                }
-                cp_async16(dst + kc * 16, static_cast<const uint8_t*>(a.kv.k_pool) + at, n);
-                cp_async16(dst + L::kHalf + vc * 16, static_cast<const uint8_t*>(a.kv.v_pool) + at, n);
+            for (int i = 0; i < kIts; ++i) {
+                const bool second = kTok == 32 && i * kPer >= 16;
+                const uint32_t kd = st + i * 512 + (k_dst ^ (k_swizzle(i * kPer) << 4));
+                const uint32_t vd = st + L::kHalf + i * 512 + (v_dst ^ (v_swizzle(i * kPer) << 4));
+                const int n = full || (e.w >> (i * kPer + lane / kChunks)) & 1 ? 16 : 0;
+                cp_async16(kd, (second ? k1 : k0) + i * 512, n);
+                cp_async16(vd, (second ? v1 : v0) + i * 512, n);
             }
             if (KV == VELO_KV_INT8 && lane < 8) {  // scales: K of both pages, V of both pages
                 const int pg = (lane >> 1) & 1, half = lane & 1;
-                const size_t at = (pg ? block1 : block0) + half * 8;
+                const size_t at = (pg ? block1 + 16 : block0) + half * 8;
                 const int n = (e.w >> (pg * 16 + half * 8)) & 0xff ? 16 : 0;
                 cp_async16(st + 2 * L::kHalf + lane * 16, (lane < 4 ? a.kv.k_scale : a.kv.v_scale) + at, n);
             }
@@ -416,25 +421,41 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_attn_kernel(con
                 }
                 // ---- softmax of this lane's tokens 8 kt + 2t, + 1 in rows g (and 8 + g)
                 float vs[kT][2];
-                float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                 for (int kt = 0; kt < kT; ++kt) {
                     float f0 = scale, f1 = scale;
-                    const int tok = kt * 8 + 2 * t;
                     if constexpr (KV == VELO_KV_INT8) {
+                        const int tok = kt * 8 + 2 * t;
                         const float2 ks = lds_half2(st + 2 * L::kHalf + tok * 2);
                         const float2 vv = lds_half2(st + 2 * L::kHalf + 2 * kTok + tok * 2);
                         f0 *= ks.x;
                         f1 *= ks.y;
-                        vs[kt][0] = (present >> tok) & 1 ? vv.x : 0.0f;
-                        vs[kt][1] = (present >> (tok + 1)) & 1 ? vv.y : 0.0f;
+                        vs[kt][0] = vv.x;
+                        vs[kt][1] = vv.y;
                     }
 #pragma unroll
                     for (int r = 0; r < R; ++r) {
-                        s[kt][2 * r] = (present >> tok) & 1 ? s[kt][2 * r] * f0 : -INFINITY;
-                        s[kt][2 * r + 1] = (present >> (tok + 1)) & 1 ? s[kt][2 * r + 1] * f1 : -INFINITY;
-                        mx[r] = fmaxf(mx[r], fmaxf(s[kt][2 * r], s[kt][2 * r + 1]));
+                        s[kt][2 * r] *= f0;
+                        s[kt][2 * r + 1] *= f1;
                     }
+                }
+                if (present != kFull) {
+#pragma unroll
+                    for (int kt = 0; kt < kT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (!((present >> (kt * 8 + 2 * t + i)) & 1)) {
+                                if constexpr (KV == VELO_KV_INT8) vs[kt][i] = 0.0f;
+#pragma unroll
+                                for (int r = 0; r < R; ++r) s[kt][2 * r + i] = -INFINITY;
+                            }
+                }
+                float mx[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    mx[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
+#pragma unroll
+                    for (int kt = 1; kt < kT; ++kt) mx[r] = fmaxf(mx[r], fmaxf(s[kt][2 * r], s[kt][2 * r + 1]));
                 }
                 float alpha[R], ref[R];
                 bool moved = false;

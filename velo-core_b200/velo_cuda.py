@@ -247,37 +247,48 @@ def _ptr(a):
     return ctypes.c_void_p(a.data_ptr())  # torch tensor
 
 
-_ELEMS = {"torch.float32": ELEM_F32, "torch.float16": ELEM_F16, "torch.bfloat16": ELEM_BF16}
-_KVS = {"torch.float16": KV_F16, "torch.int8": KV_INT8, "torch.float32": KV_F32}
+class _Types(dict):
+    """{torch dtype: code}, filled from the dtypes' names (torch is not imported here)."""
+
+    def __init__(self, **names):
+        self.names = names
+
+    def __missing__(self, dtype):
+        code = self[dtype] = self.names.get(str(dtype).removeprefix("torch."), -1)
+        return code
+
+
+_ELEMS = _Types(float32=ELEM_F32, float16=ELEM_F16, bfloat16=ELEM_BF16)
+_KVS = _Types(float16=KV_F16, int8=KV_INT8, float32=KV_F32)
+_INTS = _Types(int32=0, uint32=0)
 
 
 def _refuse(message):
     raise VeloError(ERR_INVALID_ARGUMENT, message)
 
 
-def _tensor(what, t, dtypes, shape, device, strided=False):
-    """Refuse a tensor of another element type, shape, device or layout (strided:
-    the first dimension may have any stride, the others are dense).  Returns
-    its address."""
+def _tensor(what, t, types, code, shape, device):
+    """The address of a dense tensor; refuses another element type (types[dtype]
+    must be `code`), shape, device or layout."""
     if t is None:
         _refuse(f"{what} is missing")
-    if str(t.dtype) not in dtypes:
-        _refuse(f"{what}: {t.dtype}, not {' / '.join(dtypes)}")
-    if t.shape != shape:
-        _refuse(f"{what}: shape {tuple(t.shape)}, not {shape}")
-    if t.get_device() != device:
-        _refuse(f"{what}: on {t.device}, not on the context's device {device}")
-    if not t.is_contiguous():
-        dense, step = strided, 1
-        for n, st in zip(reversed(t.shape[1:]), reversed(t.stride()[1:])):
-            dense = dense and (st == step or n == 1)
-            step *= n
-        if not dense:
-            _refuse(f"{what}: strides {t.stride()} unsupported")
+    if types[t.dtype] != code or t.shape != shape or t.get_device() != device or not t.is_contiguous():
+        _refuse(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, strides {t.stride()}: not the element type, shape "
+                f"{tuple(shape)}, device {device} or dense layout needed")
     return t.data_ptr()
 
 
-_INTS, _FLOAT = ("torch.int32", "torch.uint32"), ("torch.float32",)
+def _rows(what, t, code, shape, device):
+    """(address, row stride) of a tensor whose rows t[i] are dense and may have any
+    distance."""
+    st = t.stride()
+    if (_ELEMS[t.dtype] != code or t.shape != shape or t.get_device() != device or st[-1] != 1 or
+            (len(st) == 3 and st[1] != shape[2] and shape[1] != 1)):
+        _refuse(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, strides {st}: not the element type, shape "
+                f"{tuple(shape)}, device {device} or dense rows needed")
+    if shape[0] > 1:
+        return t.data_ptr(), st[0]
+    return t.data_ptr(), shape[1] * shape[2] if len(st) == 3 else shape[1]
 
 
 class KvCache:
@@ -293,20 +304,20 @@ class KvCache:
             _refuse(f"page_table: shape {tuple(page_table.shape)}, not [rows][max_pages]")
         pages, n_kv, _, hd = k_pool.shape
         dev = self.device = k_pool.get_device()
-        kp = _tensor("k_pool", k_pool, _KVS, k_pool.shape, dev)
-        vp = _tensor("v_pool", v_pool, (str(k_pool.dtype),), k_pool.shape, dev)
-        tb = _tensor("page_table", page_table, _INTS, page_table.shape, dev)
-        self.kv_dtype, sp = _KVS[str(k_pool.dtype)], [None, None]
-        if self.kv_dtype == KV_INT8:
-            if k_scale is None or v_scale is None:
-                _refuse("int8 pools need k_scale and v_scale")
-            sp = [_tensor(w, t, ("torch.float16",), k_pool.shape[:3], dev)
-                  for w, t in (("k_scale", k_scale), ("v_scale", v_scale))]
-        self.act = "torch.float32" if self.kv_dtype == KV_F32 else "torch.float16"
+        kv = self.kv_dtype = _KVS[k_pool.dtype]
+        if kv < 0:
+            _refuse(f"k_pool: {k_pool.dtype}, not f16, int8 or f32")
+        kp = _tensor("k_pool", k_pool, _KVS, kv, k_pool.shape, dev)
+        vp = _tensor("v_pool", v_pool, _KVS, kv, k_pool.shape, dev)
+        tb = _tensor("page_table", page_table, _INTS, 0, page_table.shape, dev)
+        ks = vs = None
+        if kv == KV_INT8:
+            ks = _tensor("k_scale", k_scale, _ELEMS, ELEM_F16, k_pool.shape[:3], dev)
+            vs = _tensor("v_scale", v_scale, _ELEMS, ELEM_F16, k_pool.shape[:3], dev)
+        self.act = ELEM_F32 if kv == KV_F32 else ELEM_F16  # of q and the outputs
         self.rows, self.n_kv, self.head_dim = page_table.shape[0], n_kv, hd
         self.tensors = (k_pool, v_pool, page_table, k_scale, v_scale)
-        self.desc = KvCacheDesc(ctypes.sizeof(KvCacheDesc), self.kv_dtype, kp, vp, sp[0], sp[1], tb, pages,
-                                page_table.shape[1], n_kv, hd)
+        self.desc = KvCacheDesc(ctypes.sizeof(KvCacheDesc), kv, kp, vp, ks, vs, tb, pages, page_table.shape[1], n_kv, hd)
         self.ref = ctypes.byref(self.desc)
 
 
@@ -324,6 +335,9 @@ class Context:
                                      ctypes.byref(h)))
         self._h = h
         self.device = device
+        self._kv_append = lib().velo_cuda_kv_append
+        self._decode_attention = lib().velo_cuda_decode_attention
+        self._token_logprobs = lib().velo_cuda_token_logprobs
 
     def close(self):
         if getattr(self, "_h", None):
@@ -431,28 +445,28 @@ class Context:
         q_out), k, v [T][n_kv][hd] f32 / f16 / bf16, rows of any stride; ctx_len
         [B] int32 cached tokens; seq_start [B+1] int32 (None: one token per
         sequence); outputs f32 for f32 pools, else f16."""
-        n, hd, dev, e = cache.n_kv, cache.head_dim, self.device, (str(k.dtype),)
-        T, B = k.shape[0], ctx_len.shape[0]
-        if cache.device != dev or cache.rows < B:
-            _refuse(f"cache: device {cache.device}, {cache.rows} page-table rows for {B} sequences on device {dev}")
-        if e[0] not in _ELEMS:
-            _refuse(f"k: {k.dtype}, not {' / '.join(_ELEMS)}")
+        n, hd, dev, act = cache.n_kv, cache.head_dim, self.device, cache.act
+        T, B, e = k.shape[0], ctx_len.shape[0], _ELEMS[k.dtype]
+        if cache.device != dev or cache.rows < B or e < 0:
+            _refuse(f"cache on device {cache.device} with {cache.rows} page-table rows, {B} sequences on device {dev}, "
+                    f"k {k.dtype}")
         pq = pqo = pko = pvo = pss = None
         ldq = Hq = 0
+        kv = (T, n, hd)
         if q is not None:
             Hq = q.shape[1]
-            pq, ldq = _tensor("q", q, e, (T, Hq, hd), dev, True), max(q.stride(0), Hq * hd) if T < 2 else q.stride(0)
-            pqo = _tensor("q_out", q_out, (cache.act,), (T, Hq, hd), dev)
-        pk, pv = _tensor("k", k, e, (T, n, hd), dev, True), _tensor("v", v, e, (T, n, hd), dev, True)
-        ldk, ldv = (k.stride(0), v.stride(0)) if T > 1 else (n * hd, n * hd)
+            heads = (T, Hq, hd)
+            pq, ldq = _rows("q", q, e, heads, dev)
+            pqo = _tensor("q_out", q_out, _ELEMS, act, heads, dev)
+        pk, ldk = _rows("k", k, e, kv, dev)
+        pv, ldv = _rows("v", v, e, kv, dev)
         if k_out is not None or v_out is not None:
-            pko = _tensor("k_out", k_out, (cache.act,), (T, n, hd), dev)
-            pvo = _tensor("v_out", v_out, (cache.act,), (T, n, hd), dev)
+            pko = _tensor("k_out", k_out, _ELEMS, act, kv, dev)
+            pvo = _tensor("v_out", v_out, _ELEMS, act, kv, dev)
         if seq_start is not None:
-            pss = _tensor("seq_start", seq_start, ("torch.int32",), (B + 1,), dev)
-        check(lib().velo_cuda_kv_append(
-            self._h, cache.ref, pq, pk, pv, _ELEMS[e[0]], ldq, ldk, ldv, pss,
-            _tensor("ctx_len", ctx_len, ("torch.int32",), (B,), dev), B, T, Hq, freq_base, pqo, pko, pvo))
+            pss = _tensor("seq_start", seq_start, _INTS, 0, (B + 1,), dev)
+        check(self._kv_append(self._h, cache.ref, pq, pk, pv, e, ldq, ldk, ldv, pss,
+                              _tensor("ctx_len", ctx_len, _INTS, 0, (B,), dev), B, T, Hq, freq_base, pqo, pko, pvo))
 
     def decode_attention_workspace(self, n_head, n_kv, head_dim):
         """Bytes of decode_attention's workspace, for any batch and lengths."""
@@ -467,17 +481,17 @@ class Context:
         f32 for f32 pools, else f16; seq_len [B] int32; lse [B][n_head] f32;
         workspace: a tensor of decode_attention_workspace bytes."""
         B, Hq, hd = shape = q.shape
-        dev = self.device
+        dev, act = self.device, cache.act
         if cache.device != dev or cache.rows < B or cache.head_dim != hd:
-            _refuse(f"cache: device {cache.device}, {cache.rows} page-table rows, head_dim {cache.head_dim} for q "
+            _refuse(f"cache on device {cache.device} with {cache.rows} page-table rows, head_dim {cache.head_dim}: q "
                     f"{tuple(shape)} on device {dev}")
-        pq = _tensor("q", q, (cache.act,), shape, dev, True)
-        po = _tensor("out", out, (cache.act,), shape, dev)
-        pl = None if lse is None else _tensor("lse", lse, _FLOAT, (B, Hq), dev)
-        pw = _tensor("workspace", workspace, (str(workspace.dtype),), workspace.shape, dev)
-        check(lib().velo_cuda_decode_attention(
-            self._h, cache.ref, pq, q.stride(0) if B > 1 else Hq * hd,
-            _tensor("seq_len", seq_len, ("torch.int32",), (B,), dev), B, Hq, scale, po, pl, pw, workspace.nbytes))
+        pq, ldq = _rows("q", q, act, shape, dev)
+        pl = None if lse is None else _tensor("lse", lse, _ELEMS, ELEM_F32, (B, Hq), dev)
+        if workspace.get_device() != dev or not workspace.is_contiguous():
+            _refuse(f"workspace: on {workspace.device} or not dense")
+        check(self._decode_attention(self._h, cache.ref, pq, ldq, _tensor("seq_len", seq_len, _INTS, 0, (B,), dev), B,
+                                     Hq, scale, _tensor("out", out, _ELEMS, act, shape, dev), pl, workspace.data_ptr(),
+                                     workspace.nbytes))
 
     def token_logprobs(self, logits, tokens, logprob, entropy=None, top_tokens=None, top_logprobs=None,
                        temperature=1.0):
@@ -486,22 +500,22 @@ class Context:
         any stride, with the entropy [M] and the n best alternatives, top_tokens
         (int32) and top_logprobs [M][n] (torch CUDA tensors, asynchronous)."""
         M, V = shape = logits.shape
-        dev = self.device
-        px = _tensor("logits", logits, _ELEMS, shape, dev, True)
+        dev, e = self.device, _ELEMS[logits.dtype]
+        if e < 0:
+            _refuse(f"logits: {logits.dtype}, not f32, f16 or bf16")
+        px, ldl = _rows("logits", logits, e, shape, dev)
         pt = pl = pe = ptt = ptl = None
-        n = 0
+        n, row = 0, (M,)
         if tokens is not None or logprob is not None:
-            pt = _tensor("tokens", tokens, _INTS, (M,), dev)
-            pl = _tensor("logprob", logprob, _FLOAT, (M,), dev)
+            pt = _tensor("tokens", tokens, _INTS, 0, row, dev)
+            pl = _tensor("logprob", logprob, _ELEMS, ELEM_F32, row, dev)
         if entropy is not None:
-            pe = _tensor("entropy", entropy, _FLOAT, (M,), dev)
+            pe = _tensor("entropy", entropy, _ELEMS, ELEM_F32, row, dev)
         if top_tokens is not None or top_logprobs is not None:
-            n = top_tokens.shape[1] if top_tokens is not None else 0
-            ptt = _tensor("top_tokens", top_tokens, _INTS, (M, n), dev)
-            ptl = _tensor("top_logprobs", top_logprobs, _FLOAT, (M, n), dev)
-        check(lib().velo_cuda_token_logprobs(
-            self._h, px, _ELEMS[str(logits.dtype)], logits.stride(0) if M > 1 else V, M, V, pt, temperature, pl, pe, n,
-            ptt, ptl))
+            n = 0 if top_tokens is None else top_tokens.shape[1]
+            ptt = _tensor("top_tokens", top_tokens, _INTS, 0, (M, n), dev)
+            ptl = _tensor("top_logprobs", top_logprobs, _ELEMS, ELEM_F32, (M, n), dev)
+        check(self._token_logprobs(self._h, px, e, ldl, M, V, pt, temperature, pl, pe, n, ptt, ptl))
 
     # ------------------------------------------------------------ model + verify
     def load_model(self, meta, tensors, shards=False):
