@@ -48,7 +48,6 @@ using sm100::smem_u32;
 constexpr int kErrSeqLen = 0x6211, kErrPage = 0x6212;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kBlocksPerSm = 2;
 constexpr int kMaxBlocks = 1024;
 constexpr int kMinUnits = 4;  // units per block at least: one per warp
 // An item of at most this many units (256 tokens of f16 pages), or of a quarter of
@@ -56,17 +55,21 @@ constexpr int kMinUnits = 4;  // units per block at least: one per warp
 constexpr int kWholeUnits = 16;
 constexpr int kRing = 64;  // unit descriptions per warp
 
+// Resident blocks per SM: INT8 pages with at most 8 query heads per KV head need
+// the third (12 warps) to cover the latency of their conversions.
+constexpr int blocks_per_sm(int kv, int R) { return kv == VELO_KV_INT8 && R == 1 ? 3 : 2; }
+
 constexpr int tokens_of(int kv) { return kv == VELO_KV_F16 ? 16 : kv == VELO_KV_INT8 ? 32 : 8; }
 constexpr int bytes_of(int kv) { return kv == VELO_KV_F16 ? 2 : kv == VELO_KV_INT8 ? 1 : 4; }
 
 // Shared memory of a block; the lengths and the prefix sums follow.
-template <int KV, int D>
+template <int KV, int D, int R>
 struct Layout {
     static constexpr int kTok = tokens_of(KV);
     static constexpr int kRow = D * bytes_of(KV);               // bytes of a token's K or V
     static constexpr int kHalf = kTok * kRow;                   // K, then V
     static constexpr int kStage = 2 * kHalf + (KV == VELO_KV_INT8 ? 4 * kTok : 0);  // + scales
-    static constexpr int kStages = D == 128 ? 3 : 6;
+    static constexpr int kStages = (blocks_per_sm(KV, R) == 3 ? 2 : 3) * (128 / D);
     static constexpr int kRings = kWarps * kStages * kStage;
     static constexpr int kStats = kRings + kWarps * kRing * 16;
     static constexpr int kQ = kStats + 3 * kWarps * 16 * 4;     // f32: q, and each warp's weights
@@ -119,12 +122,12 @@ __device__ __forceinline__ float2 lds_half2(uint32_t addr) {
     return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -199,8 +202,8 @@ __device__ __forceinline__ int cut(const int* pre, int B, int per_seq, int total
 
 // KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item.
 template <int KV, int D, int R>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) decode_attn_kernel(const DecodeAttnArgs a, const Plan plan) {
-    using L = Layout<KV, D>;
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_kernel(const DecodeAttnArgs a, const Plan plan) {
+    using L = Layout<KV, D, R>;
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
     constexpr int kTok = L::kTok, S = L::kStages, kRows = 8 * R;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -783,14 +786,14 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnA
 }
 
 template <int KV, int D, int R>
-cudaError_t launch_typed(const DecodeAttnArgs& a, int blocks, cudaStream_t s) {
-    using L = Layout<KV, D>;
+cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
+    using L = Layout<KV, D, R>;
     static SmemAttr attr;
     const int smem = L::kLens + (2 * a.B + 1) * 4;
     cudaError_t e = ensure_smem(attr, decode_attn_kernel<KV, D, R>, smem);
     if (e != cudaSuccess) return e;
     Plan p;
-    p.blocks = blocks;
+    const int blocks = p.blocks = std::min(blocks_per_sm(KV, R) * sm_count, kMaxBlocks);
     p.group = a.Hq / a.kv.n_kv;
     p.tiles = (p.group + 8 * R - 1) / (8 * R);
     decode_attn_kernel<KV, D, R><<<blocks, kThreads, smem, s>>>(a, p);
@@ -811,27 +814,27 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int blocks, cudaStream_t s) {
 }
 
 template <int KV, int R>
-cudaError_t launch_rows(const DecodeAttnArgs& a, int blocks, cudaStream_t s) {
-    return a.kv.head_dim == 64 ? launch_typed<KV, 64, R>(a, blocks, s) : launch_typed<KV, 128, R>(a, blocks, s);
+cudaError_t launch_rows(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
+    return a.kv.head_dim == 64 ? launch_typed<KV, 64, R>(a, sm_count, s) : launch_typed<KV, 128, R>(a, sm_count, s);
 }
 
-int grid_blocks(int sm_count) { return std::min(kBlocksPerSm * sm_count, kMaxBlocks); }
 // tiles of 8 query heads per item: f32 items hold 8 heads, the others up to 16
 int row_tiles(int group, int kv_dtype) { return kv_dtype != VELO_KV_F32 && group > 8 ? 2 : 1; }
 
 }  // namespace
 
 size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
-    const size_t blocks = grid_blocks(sm_count);
-    return blocks * sizeof(int4) + 2 * blocks * slot_floats(8 * row_tiles(Hq / Hkv, VELO_KV_F16), D) * sizeof(float);
+    const int R = row_tiles(Hq / Hkv, VELO_KV_INT8);  // the most blocks and the most rows of any page type
+    const size_t blocks = std::min(blocks_per_sm(VELO_KV_INT8, R) * sm_count, kMaxBlocks);
+    return blocks * sizeof(int4) + 2 * blocks * slot_floats(8 * R, D) * sizeof(float);
 }
 
 cudaError_t launch_decode_attention(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
-    const int blocks = grid_blocks(sm_count), R = row_tiles(a.Hq / a.kv.n_kv, a.kv.kv_dtype);
-    if (a.kv.kv_dtype == VELO_KV_F32) return launch_rows<VELO_KV_F32, 1>(a, blocks, s);
+    const int R = row_tiles(a.Hq / a.kv.n_kv, a.kv.kv_dtype);
+    if (a.kv.kv_dtype == VELO_KV_F32) return launch_rows<VELO_KV_F32, 1>(a, sm_count, s);
     if (a.kv.kv_dtype == VELO_KV_INT8)
-        return R == 2 ? launch_rows<VELO_KV_INT8, 2>(a, blocks, s) : launch_rows<VELO_KV_INT8, 1>(a, blocks, s);
-    return R == 2 ? launch_rows<VELO_KV_F16, 2>(a, blocks, s) : launch_rows<VELO_KV_F16, 1>(a, blocks, s);
+        return R == 2 ? launch_rows<VELO_KV_INT8, 2>(a, sm_count, s) : launch_rows<VELO_KV_INT8, 1>(a, sm_count, s);
+    return R == 2 ? launch_rows<VELO_KV_F16, 2>(a, sm_count, s) : launch_rows<VELO_KV_F16, 1>(a, sm_count, s);
 }
 
 }  // namespace velo
