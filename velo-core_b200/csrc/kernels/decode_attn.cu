@@ -116,10 +116,17 @@ __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ float2 lds_half2(uint32_t addr) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+__device__ __forceinline__ float lds_half(uint32_t addr) {
+    uint16_t v;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
+    return __half2float(__ushort_as_half(v));
+}
+// The 8 x 8 matrix of 16-bit elements a warp holds (lane 4 row + t: columns 2t,
+// 2t + 1), transposed.
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -354,36 +361,40 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
         const int h0 = hk * plan.group + tile * kRows, nh = min(kRows, plan.group - tile * kRows);
         const Act* qp = static_cast<const Act*>(a.q) + (size_t)x.b * a.ldq + (size_t)h0 * D;
 
-        // ---- running state: row = 8r + g (f32: rows 2t, 2t + 1 of this lane's token)
-        constexpr int kM = KV == VELO_KV_F32 ? 2 : R;
-        float m[kM], l[kM];
+        // ---- running state.  Tensor cores: scores and output are held transposed (keys or
+        // dimensions x heads), so a lane has heads 8r + 2t + {0, 1}; f32: heads 2t + {0, 1} of
+        // its token.  m is the reference of the weights, at most 2^8 below the largest.
+        constexpr int kH = KV == VELO_KV_F32 ? 1 : R;
+        float m[kH][2], l[kH][2];
 #pragma unroll
-        for (int r = 0; r < kM; ++r) {
-            m[r] = -INFINITY;
-            l[r] = 0.0f;
-        }
-        constexpr int kN = KV == VELO_KV_F32 ? 1 : D / 8;       // output tiles of 8 dimensions
-        float o[KV == VELO_KV_F32 ? 1 : R][kN][4] = {};
+        for (int r = 0; r < kH; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                m[r][e] = -INFINITY;
+                l[r][e] = 0.0f;
+            }
+        constexpr int kN = KV == VELO_KV_F32 ? 1 : D / 16;      // output tiles of 16 dimensions
+        float o[kH][kN][4] = {};
         constexpr int kO = KV == VELO_KV_F32 ? D / 32 : 1;      // dimensions per lane
         float of[KV == VELO_KV_F32 ? 8 : 1][kO] = {};
-        uint32_t qa[KV == VELO_KV_F32 ? 1 : D / 16][4];
+        uint32_t qb[kH][KV == VELO_KV_F32 ? 1 : D / 16][2];     // q as B fragments: head 8r + g
         if constexpr (KV == VELO_KV_F32) {
             float* qs = reinterpret_cast<float*>(smem + L::kQ);
             for (int i = tid; i < 8 * D; i += kThreads) qs[i] = i / D < nh ? to_f32(qp[i]) : 0.0f;
             __syncthreads();
         } else {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks) {
-                // the dimensions a lane holds of contraction step ks: ldmatrix's own order for
-                // f16, 4 of its 16 consecutive bytes for int8
-                const int d0 = KV == VELO_KV_F16 ? 16 * ks + 2 * t : 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
-                const int d1 = d0 + (KV == VELO_KV_F16 ? 8 : 2);
+            for (int r = 0; r < R; ++r) {
+                const int row = 8 * r + g;
+                const Act* qr = qp + (size_t)row * D;
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    const int row = 8 * r + g;
-                    const bool live = r < R && row < nh;
-                    qa[ks][r] = live ? *reinterpret_cast<const uint32_t*>(qp + (size_t)row * D + d0) : 0u;
-                    qa[ks][2 + r] = live ? *reinterpret_cast<const uint32_t*>(qp + (size_t)row * D + d1) : 0u;
+                for (int ks = 0; ks < D / 16; ++ks) {
+                    // the dimensions a lane holds of contraction step ks: ldmatrix's own order for
+                    // f16, 4 of its 16 consecutive bytes for int8
+                    const int d0 = KV == VELO_KV_F16 ? 16 * ks + 2 * t : 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
+                    const int d1 = d0 + (KV == VELO_KV_F16 ? 8 : 2);
+                    qb[r][ks][0] = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d0) : 0u;
+                    qb[r][ks][1] = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d1) : 0u;
                 }
             }
         }
@@ -395,127 +406,150 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
             const uint32_t st = stage0 + (j % S) * L::kStage;
             const uint32_t present = ring[j % kRing].w;
             if constexpr (KV != VELO_KV_F32) {
-                // ---- scores
-                constexpr int kT = kTok / 8;
-                float s[kT][4] = {};
-                if constexpr (KV == VELO_KV_F16) {
-                    const int r = lane & 7, mi = lane >> 3;
-                    const uint32_t kb = st + ((mi >> 1) * 8 + r) * L::kRow;
+                // ---- scores of 16 kt + {g, 8 + g}: two accumulators each, to halve the chain
+                constexpr int kT = kTok / 16;
+                float s[kT][R][4];
+                {
+                    float sum[2][kT][R][4] = {};
+                    if constexpr (KV == VELO_KV_F16) {
+                        const int r8 = lane & 7, mi = lane >> 3;
+                        const uint32_t kb = st + ((mi & 1) * 8 + r8) * L::kRow;
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        uint32_t kf[4];
-                        ldmatrix_x4(kf, kb + (((2 * ks + (mi & 1)) ^ r) << 4));
-                        mma_f16(s[0], qa[ks], kf[0], kf[1]);
-                        mma_f16(s[1], qa[ks], kf[2], kf[3]);
-                    }
-                } else {
+                        for (int ks = 0; ks < D / 16; ++ks) {
+                            uint32_t kf[4];
+                            ldmatrix_x4(kf, kb + (((2 * ks + (mi >> 1)) ^ r8) << 4));
 #pragma unroll
-                    for (int h = 0; h < D / 64; ++h)
-#pragma unroll
-                        for (int kt = 0; kt < kT; ++kt) {
-                            const int row = kt * 8 + g, ch = (4 * h + t) ^ (D == 128 ? (row & 1) << 2 : 0);
-                            const uint4 w4 = lds128(st + row * L::kRow + ch * 16);
-                            const uint32_t w[4] = {w4.x ^ 0x80808080u, w4.y ^ 0x80808080u, w4.z ^ 0x80808080u,
-                                                   w4.w ^ 0x80808080u};
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                mma_f16(s[kt], qa[4 * h + i], bytes_to_f16<0>(w[i]), bytes_to_f16<1>(w[i]));
+                            for (int r = 0; r < R; ++r) mma_f16(sum[ks & 1][0][r], kf, qb[r][ks][0], qb[r][ks][1]);
                         }
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                            for (int kt = 0; kt < kT; ++kt) {
+                                uint32_t w[2][4];  // 16 bytes of tokens g and 8 + g
+#pragma unroll
+                                for (int i = 0; i < 2; ++i) {
+                                    const int row = kt * 16 + 8 * i + g, ch = (4 * h + t) ^ (D == 128 ? (row & 1) << 2 : 0);
+                                    const uint4 v = lds128(st + row * L::kRow + ch * 16);
+                                    w[i][0] = v.x ^ 0x80808080u;
+                                    w[i][1] = v.y ^ 0x80808080u;
+                                    w[i][2] = v.z ^ 0x80808080u;
+                                    w[i][3] = v.w ^ 0x80808080u;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const uint32_t kf[4] = {bytes_to_f16<0>(w[0][i]), bytes_to_f16<0>(w[1][i]),
+                                                            bytes_to_f16<1>(w[0][i]), bytes_to_f16<1>(w[1][i])};
+#pragma unroll
+                                    for (int r = 0; r < R; ++r)
+                                        mma_f16(sum[i & 1][kt][r], kf, qb[r][4 * h + i][0], qb[r][4 * h + i][1]);
+                                }
+                            }
+                    }
+#pragma unroll
+                    for (int kt = 0; kt < kT; ++kt)
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[kt][r][e] = sum[0][kt][r][e] + sum[1][kt][r][e];
                 }
-                // ---- softmax of this lane's tokens 8 kt + 2t, + 1 in rows g (and 8 + g)
+                // ---- weights: element 2i + e is token 16 kt + 8i + g, head 8r + 2t + e
                 float vs[kT][2];
 #pragma unroll
-                for (int kt = 0; kt < kT; ++kt) {
-                    float f0 = scale, f1 = scale;
-                    if constexpr (KV == VELO_KV_INT8) {
-                        const int tok = kt * 8 + 2 * t;
-                        const float2 ks = lds_half2(st + 2 * L::kHalf + tok * 2);
-                        const float2 vv = lds_half2(st + 2 * L::kHalf + 2 * kTok + tok * 2);
-                        f0 *= ks.x;
-                        f1 *= ks.y;
-                        vs[kt][0] = vv.x;
-                        vs[kt][1] = vv.y;
-                    }
+                for (int kt = 0; kt < kT; ++kt)
 #pragma unroll
-                    for (int r = 0; r < R; ++r) {
-                        s[kt][2 * r] *= f0;
-                        s[kt][2 * r + 1] *= f1;
+                    for (int i = 0; i < 2; ++i) {
+                        float f = scale;
+                        if constexpr (KV == VELO_KV_INT8) {
+                            const uint32_t at = st + 2 * L::kHalf + (kt * 16 + 8 * i + g) * 2;
+                            f *= lds_half(at);
+                            vs[kt][i] = lds_half(at + 2 * kTok);
+                        }
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            s[kt][r][2 * i] *= f;
+                            s[kt][r][2 * i + 1] *= f;
+                        }
                     }
-                }
                 if (present != kFull) {
 #pragma unroll
                     for (int kt = 0; kt < kT; ++kt)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            if (!((present >> (kt * 8 + 2 * t + i)) & 1)) {
+                            if (!((present >> (kt * 16 + 8 * i + g)) & 1)) {
                                 if constexpr (KV == VELO_KV_INT8) vs[kt][i] = 0.0f;
 #pragma unroll
-                                for (int r = 0; r < R; ++r) s[kt][2 * r + i] = -INFINITY;
+                                for (int r = 0; r < R; ++r) s[kt][r][2 * i] = s[kt][r][2 * i + 1] = -INFINITY;
                             }
                 }
-                float mx[R];
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    mx[r] = fmaxf(s[0][2 * r], s[0][2 * r + 1]);
-#pragma unroll
-                    for (int kt = 1; kt < kT; ++kt) mx[r] = fmaxf(mx[r], fmaxf(s[kt][2 * r], s[kt][2 * r + 1]));
-                }
-                float alpha[R], ref[R];
                 bool moved = false;
+                float top[R][2];
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
-                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
-                    const float mn = fmaxf(m[r], mx[r]);
-                    ref[r] = mn == -INFINITY ? 0.0f : mn;
-                    alpha[r] = ex2_approx(m[r] - ref[r]);
-                    moved |= mn != m[r];
-                    m[r] = mn;
-                    l[r] *= alpha[r];
-                }
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float mx = fmaxf(s[0][r][e], s[0][r][2 + e]);
+#pragma unroll
+                        for (int kt = 1; kt < kT; ++kt) mx = fmaxf(mx, fmaxf(s[kt][r][e], s[kt][r][2 + e]));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                        top[r][e] = mx;
+                        moved |= mx > m[r][e] + 8.0f;
+                    }
                 if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int n = 0; n < kN; ++n)
+                        for (int e = 0; e < 2; ++e) {
+                            const float mn = fmaxf(m[r][e], top[r][e]);
+                            const float alpha = mn == m[r][e] ? 1.0f : ex2_approx(m[r][e] - mn);
+                            m[r][e] = mn;
+                            l[r][e] *= alpha;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) o[r][n][e] *= alpha[r];
+                            for (int n = 0; n < kN; ++n) {
+                                o[r][n][e] *= alpha;
+                                o[r][n][2 + e] *= alpha;
+                            }
+                        }
                 }
-                // ---- weights as A fragments (rows g: the value, rows 8 + g: its remainder) and P V
+                // ---- the weights, as value and remainder, become B fragments by transposition; P V
 #pragma unroll
-                for (int kk = 0; kk < kT / 2; ++kk) {
-                    uint32_t pa[R][4];
+                for (int kt = 0; kt < kT; ++kt) {
+                    uint32_t hi[R][2], lo[R][2];
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float p0 = ex2_approx(s[2 * kk + i][2 * r] - ref[r]);
-                            float p1 = ex2_approx(s[2 * kk + i][2 * r + 1] - ref[r]);
-                            l[r] += p0 + p1;
+                            const float r0 = m[r][0] == -INFINITY ? 0.0f : m[r][0], r1 = m[r][1] == -INFINITY ? 0.0f : m[r][1];
+                            const float p0 = ex2_approx(s[kt][r][2 * i] - r0), p1 = ex2_approx(s[kt][r][2 * i + 1] - r1);
+                            l[r][0] += p0;
+                            l[r][1] += p1;
                             if constexpr (KV == VELO_KV_INT8)
-                                split_bf16(p0 * vs[2 * kk + i][0], p1 * vs[2 * kk + i][1], pa[r][2 * i], pa[r][2 * i + 1]);
+                                split_bf16(p0 * vs[kt][i], p1 * vs[kt][i], hi[r][i], lo[r][i]);
                             else
-                                split_f16(p0, p1, pa[r][2 * i], pa[r][2 * i + 1]);
+                                split_f16(p0, p1, hi[r][i], lo[r][i]);
+                            hi[r][i] = transpose8x8(hi[r][i]);
+                            lo[r][i] = transpose8x8(lo[r][i]);
                         }
                     if constexpr (KV == VELO_KV_F16) {
                         const int r8 = lane & 7, mi = lane >> 3;
-                        const uint32_t vb = st + L::kHalf + ((mi & 1) * 8 + r8) * L::kRow;
+                        const uint32_t vb = st + L::kHalf + ((mi >> 1) * 8 + r8) * L::kRow;
 #pragma unroll
-                        for (int n = 0; n < D / 16; ++n) {
+                        for (int n = 0; n < kN; ++n) {
                             uint32_t vf[4];
-                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi >> 1)) ^ r8) << 4));
+                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi & 1)) ^ r8) << 4));
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                mma_f16(o[r][2 * n], pa[r], vf[0], vf[1]);
-                                mma_f16(o[r][2 * n + 1], pa[r], vf[2], vf[3]);
+                                mma_f16(o[r][n], vf, hi[r][0], hi[r][1]);
+                                mma_f16(o[r][n], vf, lo[r][0], lo[r][1]);
                             }
                         }
                     } else {
-                        // dimension n of this lane's column: g * D / 8 + n
+                        // rows g and 8 + g of tile n: dimensions g * D / 8 + 2n and + 1
                         uint32_t w[4][D / 32];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int row = kk * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
+                            const int row = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
                             const uint32_t rb = st + L::kHalf + row * L::kRow;
                             if constexpr (D == 128) {
                                 const uint4 v = lds128(rb + ((g ^ (row & 6)) << 4));
@@ -530,17 +564,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             }
                         }
 #pragma unroll
-                        for (int q4 = 0; q4 < D / 32; ++q4) {
+                        for (int n = 0; n < kN; n += 2) {
+                            const int q4 = n / 2;
+                            const uint32_t va[4] = {byte_pair_to_bf16<0>(w[0][q4], w[1][q4]), byte_pair_to_bf16<1>(w[0][q4], w[1][q4]),
+                                                    byte_pair_to_bf16<0>(w[2][q4], w[3][q4]), byte_pair_to_bf16<1>(w[2][q4], w[3][q4])};
+                            const uint32_t vb[4] = {byte_pair_to_bf16<2>(w[0][q4], w[1][q4]), byte_pair_to_bf16<3>(w[0][q4], w[1][q4]),
+                                                    byte_pair_to_bf16<2>(w[2][q4], w[3][q4]), byte_pair_to_bf16<3>(w[2][q4], w[3][q4])};
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                mma_bf16(o[r][4 * q4], pa[r], byte_pair_to_bf16<0>(w[0][q4], w[1][q4]),
-                                         byte_pair_to_bf16<0>(w[2][q4], w[3][q4]));
-                                mma_bf16(o[r][4 * q4 + 1], pa[r], byte_pair_to_bf16<1>(w[0][q4], w[1][q4]),
-                                         byte_pair_to_bf16<1>(w[2][q4], w[3][q4]));
-                                mma_bf16(o[r][4 * q4 + 2], pa[r], byte_pair_to_bf16<2>(w[0][q4], w[1][q4]),
-                                         byte_pair_to_bf16<2>(w[2][q4], w[3][q4]));
-                                mma_bf16(o[r][4 * q4 + 3], pa[r], byte_pair_to_bf16<3>(w[0][q4], w[1][q4]),
-                                         byte_pair_to_bf16<3>(w[2][q4], w[3][q4]));
+                                mma_bf16(o[r][n], va, hi[r][0], hi[r][1]);
+                                mma_bf16(o[r][n + 1], vb, hi[r][0], hi[r][1]);
+                                mma_bf16(o[r][n], va, lo[r][0], lo[r][1]);
+                                mma_bf16(o[r][n + 1], vb, lo[r][0], lo[r][1]);
                             }
                         }
                     }
@@ -580,11 +615,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                     float mx = sv;
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                    const float mn = fmaxf(m[r], mx), rf = mn == -INFINITY ? 0.0f : mn;
-                    const float al = ex2_approx(m[r] - rf), p = ex2_approx(sv - rf);
-                    moved |= mn != m[r];
-                    m[r] = mn;
-                    l[r] = l[r] * al + p;
+                    const float mn = fmaxf(m[0][r], mx), rf = mn == -INFINITY ? 0.0f : mn;
+                    const float al = ex2_approx(m[0][r] - rf), p = ex2_approx(sv - rf);
+                    moved |= mn != m[0][r];
+                    m[0][r] = mn;
+                    l[0][r] = l[0][r] * al + p;
                     pw[g * 8 + 2 * t + r] = p;
                     if (g == 0) pw[64 + 2 * t + r] = al;
                 }
@@ -625,29 +660,17 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
         // ---- the item's end in this range: the warps' states into one.  A warp's output goes
         // into the stage it has just read, which is refilled after the join.
         const uint32_t buf = stage0 + ((j + S - 1) % S) * L::kStage;  // stage of unit j - 1
-        if constexpr (KV == VELO_KV_F32) {
 #pragma unroll
-            for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < kH; ++r)
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], d);
-            if (g == 0) {
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                for (int r = 0; r < 2; ++r) {
-                    stat_m[warp * 16 + 2 * t + r] = m[r];
-                    stat_l[warp * 16 + 2 * t + r] = l[r];
+                for (int d = 4; d < 32; d <<= 1) l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], d);
+                if (g == 0) {
+                    stat_m[warp * 16 + 8 * r + 2 * t + e] = m[r][e];
+                    stat_l[warp * 16 + 8 * r + 2 * t + e] = l[r][e];
                 }
             }
-        } else {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-                if (t == 0) {
-                    stat_m[warp * 16 + 8 * r + g] = m[r];
-                    stat_l[warp * 16 + 8 * r + g] = l[r];
-                }
-            }
-        }
         if (lane == 0) stat_buf[warp] = (int)(buf - smem_u32(smem));
         if (pending) {
             float* dst = reinterpret_cast<float*>(smem + (buf - smem_u32(smem)));
@@ -657,13 +680,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
 #pragma unroll
                     for (int e = 0; e < kO; ++e) dst[h * D + lane * kO + e] = of[h][e];
             } else {
-                // fragment order [row][tile][8 columns], tiles XORed with the row against bank conflicts
+                // [head][fragment row], eights XORed with the head against bank conflicts
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
                     for (int n = 0; n < kN; ++n)
-                        *reinterpret_cast<float2*>(dst + (8 * r + g) * D + ((n ^ g) << 3) + 2 * t) =
-                            make_float2(o[r][n][0] + o[r][n][2], o[r][n][1] + o[r][n][3]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] = o[r][n][e];
             }
         }
         __syncthreads();
@@ -681,18 +705,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                 if (lw == 0.0f) continue;  // nothing from this warp (its buffer is in flight)
                 const float f = ex2_approx(stat_m[w * 16 + row] - M);
                 const float* src = reinterpret_cast<const float*>(smem + stat_buf[w]) + row * D;
+                const int flip = KV == VELO_KV_F32 ? 0 : (row >> 1 & 3) << 3;
                 float v0, v1;
-                if constexpr (KV == VELO_KV_F32) {
-                    v0 = src[d];
-                    v1 = src[d + 1];
-                } else if constexpr (KV == VELO_KV_F16) {
-                    const float2 v = *reinterpret_cast<const float2*>(src + ((d >> 3 ^ (row & 7)) << 3) + (d & 7));
+                if constexpr (KV == VELO_KV_INT8) {  // dimension gg D / 8 + 2n + half is fragment row 16n + 8 half + gg
+                    const int at = 8 * (d % (D / 8)) + d / (D / 8);
+                    v0 = src[at ^ flip];
+                    v1 = src[(at + 8) ^ flip];
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(src + (d ^ flip));
                     v0 = v.x;
                     v1 = v.y;
-                } else {  // dimension = column * D / 8 + tile
-                    const int col = d / (D / 8), n = d % (D / 8);
-                    v0 = src[((n ^ (row & 7)) << 3) + col];
-                    v1 = src[(((n + 1) ^ (row & 7)) << 3) + col];
                 }
                 Ls = fmaf(lw, f, Ls);
                 y0 = fmaf(v0, f, y0);
