@@ -133,12 +133,6 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
 // Two f32 as a pair of 16-bit parts and the pair of their remainders.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -147,31 +141,15 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ void split_bf16(float x, float y, uint32_t& hi, uint32_t& lo) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(x - __bfloat162float(h.x), y - __bfloat162float(h.y));
-    hi = *reinterpret_cast<const uint32_t*>(&h);
-    lo = *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// Bytes 2i and 2i + 1 of w (int8 with the sign bit flipped) as an exact f16
-// pair: 0x6400 | u is 1024 + u.
-template <int i>
-__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t w) {
-    uint32_t v = __byte_perm(w, 0x64646464u, i ? 0x4342 : 0x4140);
-    const uint32_t bias = 0x64806480u;  // 1152
+// The even (odd) bytes of w, int8, as an exact f16 pair: 0x6400 | u is 1024 + u,
+// u = the byte with its sign bit flipped, and 1152 comes off again.
+__device__ __forceinline__ uint32_t even_bytes_f16(uint32_t w) {
+    uint32_t v = (w & 0x00ff00ffu) ^ 0x64806480u;
+    const uint32_t bias = 0x64806480u;
     const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-// Bytes b of the words w0 and w1 (int8) as an exact bf16 pair: 0x4300 | low 7
-// bits is 128 + them, 0x4300 | sign bit is 128 or 256.
-template <int b>
-__device__ __forceinline__ uint32_t byte_pair_to_bf16(uint32_t w0, uint32_t w1) {
-    const uint32_t x = __byte_perm(w0, w1, b | b << 4 | (4 + b) << 8 | (4 + b) << 12);  // odd bytes are masked out
-    uint32_t v = (x & 0x007f007fu) | 0x43004300u, s = (x & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<__nv_bfloat162*>(&v), *reinterpret_cast<__nv_bfloat162*>(&s));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
+__device__ __forceinline__ uint32_t odd_bytes_f16(uint32_t w) { return even_bytes_f16(w >> 8); }
 
 // The largest b with pre[b] <= u.
 __device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
@@ -311,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
         return KV == VELO_KV_F16 ? row & 7 : KV == VELO_KV_INT8 && D == 64 ? 0 : (row & 1) << 2;
     };
     auto v_swizzle = [](int row) {
-        return KV == VELO_KV_F16 ? row & 7 : KV == VELO_KV_F32 ? 0 : D == 128 ? row & 6 : (row >> 1) & 3;
+        return KV == VELO_KV_F32 ? 0 : KV == VELO_KV_INT8 && D == 64 ? (row >> 1) & 3 : row & 7;
     };
     const uint32_t k_dst = lane / kChunks * L::kRow + (((lane % kChunks) ^ k_swizzle(lane / kChunks)) << 4);
     const uint32_t v_dst = lane / kChunks * L::kRow + (((lane % kChunks) ^ v_swizzle(lane / kChunks)) << 4);
@@ -390,14 +368,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
                     // the dimensions a lane holds of contraction step ks: ldmatrix's own order for
-                    // f16, 4 of its 16 consecutive bytes for int8
+                    // f16; the even, then the odd ones of 4 consecutive bytes for int8
                     const int d0 = KV == VELO_KV_F16 ? 16 * ks + 2 * t : 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
                     const int d1 = d0 + (KV == VELO_KV_F16 ? 8 : 2);
-                    qb[r][ks][0] = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d0) : 0u;
-                    qb[r][ks][1] = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d1) : 0u;
+                    uint32_t x = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d0) : 0u;
+                    uint32_t y = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d1) : 0u;
+                    qb[r][ks][0] = KV == VELO_KV_F16 ? x : __byte_perm(x, y, 0x5410);
+                    qb[r][ks][1] = KV == VELO_KV_F16 ? y : __byte_perm(x, y, 0x7632);
                 }
             }
         }
+        // INT8: the weights times the V scales are kept within f16 by a power of two that brings
+        // the largest scale seen to 2^5 .. 2^6 (0: none yet)
+        float v_unit = 0.0f;
         bool pending = false;
         for (; j < n_w && u0 + warp + kWarps * j < seg_end; ++j) {
             if (pending) issue(j - 1 + S);
@@ -431,15 +414,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                                 for (int i = 0; i < 2; ++i) {
                                     const int row = kt * 16 + 8 * i + g, ch = (4 * h + t) ^ (D == 128 ? (row & 1) << 2 : 0);
                                     const uint4 v = lds128(st + row * L::kRow + ch * 16);
-                                    w[i][0] = v.x ^ 0x80808080u;
-                                    w[i][1] = v.y ^ 0x80808080u;
-                                    w[i][2] = v.z ^ 0x80808080u;
-                                    w[i][3] = v.w ^ 0x80808080u;
+                                    w[i][0] = v.x;
+                                    w[i][1] = v.y;
+                                    w[i][2] = v.z;
+                                    w[i][3] = v.w;
                                 }
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const uint32_t kf[4] = {bytes_to_f16<0>(w[0][i]), bytes_to_f16<0>(w[1][i]),
-                                                            bytes_to_f16<1>(w[0][i]), bytes_to_f16<1>(w[1][i])};
+                                    const uint32_t kf[4] = {even_bytes_f16(w[0][i]), even_bytes_f16(w[1][i]),
+                                                            odd_bytes_f16(w[0][i]), odd_bytes_f16(w[1][i])};
 #pragma unroll
                                     for (int r = 0; r < R; ++r)
                                         mma_f16(sum[i & 1][kt][r], kf, qb[r][4 * h + i][0], qb[r][4 * h + i][1]);
@@ -483,6 +466,27 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             }
                 }
                 bool moved = false;
+                if constexpr (KV == VELO_KV_INT8) {
+                    float big = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                    if (big * v_unit > 64.0f || v_unit == 0.0f) {  // the same for the whole warp
+                        // 2^5 / the power of two below the largest scale (f16: at least 2^-24)
+                        const float unit = big > 0.0f ? __uint_as_float((254u + 5u << 23) - (__float_as_uint(big) & 0x7f800000u)) : 0.0f;
+                        const float f = unit * (v_unit > 0.0f ? 1.0f / v_unit : 0.0f);
+                        v_unit = unit;
+#pragma unroll
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[r][n][e] *= f;
+                    }
+#pragma unroll
+                    for (int kt = 0; kt < kT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) vs[kt][i] *= v_unit;
+                }
                 float top[R][2];
 #pragma unroll
                 for (int r = 0; r < R; ++r)
@@ -524,20 +528,18 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             const float p0 = ex2_approx(s[kt][r][2 * i] - r0), p1 = ex2_approx(s[kt][r][2 * i + 1] - r1);
                             l[r][0] += p0;
                             l[r][1] += p1;
-                            if constexpr (KV == VELO_KV_INT8)
-                                split_bf16(p0 * vs[kt][i], p1 * vs[kt][i], hi[r][i], lo[r][i]);
-                            else
-                                split_f16(p0, p1, hi[r][i], lo[r][i]);
+                            const float v = KV == VELO_KV_INT8 ? vs[kt][i] : 1.0f;
+                            split_f16(p0 * v, p1 * v, hi[r][i], lo[r][i]);
                             hi[r][i] = transpose8x8(hi[r][i]);
                             lo[r][i] = transpose8x8(lo[r][i]);
                         }
+                    const int r8 = lane & 7, mi = lane >> 3, row = kt * 16 + (mi >> 1) * 8 + r8;
+                    const uint32_t vb = st + L::kHalf + row * L::kRow, flip = v_swizzle(row);
                     if constexpr (KV == VELO_KV_F16) {
-                        const int r8 = lane & 7, mi = lane >> 3;
-                        const uint32_t vb = st + L::kHalf + ((mi >> 1) * 8 + r8) * L::kRow;
 #pragma unroll
                         for (int n = 0; n < kN; ++n) {
                             uint32_t vf[4];
-                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi & 1)) ^ r8) << 4));
+                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi & 1)) ^ flip) << 4));
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
                                 mma_f16(o[r][n], vf, hi[r][0], hi[r][1]);
@@ -545,37 +547,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             }
                         }
                     } else {
-                        // rows g and 8 + g of tile n: dimensions g * D / 8 + 2n and + 1
-                        uint32_t w[4][D / 32];
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int row = kt * 16 + 2 * t + (i & 1) + (i >> 1) * 8;
-                            const uint32_t rb = st + L::kHalf + row * L::kRow;
-                            if constexpr (D == 128) {
-                                const uint4 v = lds128(rb + ((g ^ (row & 6)) << 4));
-                                w[i][0] = v.x;
-                                w[i][1] = v.y;
-                                w[i][2] = v.z;
-                                w[i][3] = v.w;
-                            } else {
-                                const uint2 v = lds64(rb + ((((g >> 1) ^ ((row >> 1) & 3)) << 4) | (g & 1) << 3));
-                                w[i][0] = v.x;
-                                w[i][1] = v.y;
-                            }
-                        }
+                        // transposed as 16-bit units, a register holds two dimensions of two tokens:
+                        // row 8 half + g of tile n is dimension 32 (n / 2) + 16 half + 2 g + n % 2
 #pragma unroll
                         for (int n = 0; n < kN; n += 2) {
-                            const int q4 = n / 2;
-                            const uint32_t va[4] = {byte_pair_to_bf16<0>(w[0][q4], w[1][q4]), byte_pair_to_bf16<1>(w[0][q4], w[1][q4]),
-                                                    byte_pair_to_bf16<0>(w[2][q4], w[3][q4]), byte_pair_to_bf16<1>(w[2][q4], w[3][q4])};
-                            const uint32_t vb[4] = {byte_pair_to_bf16<2>(w[0][q4], w[1][q4]), byte_pair_to_bf16<3>(w[0][q4], w[1][q4]),
-                                                    byte_pair_to_bf16<2>(w[2][q4], w[3][q4]), byte_pair_to_bf16<3>(w[2][q4], w[3][q4])};
+                            uint32_t w[4];
+                            ldmatrix_x4_trans(w, vb + (((n + (mi & 1)) ^ flip) << 4));
+                            const uint32_t va[4] = {even_bytes_f16(w[0]), even_bytes_f16(w[1]), even_bytes_f16(w[2]), even_bytes_f16(w[3])};
+                            const uint32_t vo[4] = {odd_bytes_f16(w[0]), odd_bytes_f16(w[1]), odd_bytes_f16(w[2]), odd_bytes_f16(w[3])};
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                mma_bf16(o[r][n], va, hi[r][0], hi[r][1]);
-                                mma_bf16(o[r][n + 1], vb, hi[r][0], hi[r][1]);
-                                mma_bf16(o[r][n], va, lo[r][0], lo[r][1]);
-                                mma_bf16(o[r][n + 1], vb, lo[r][0], lo[r][1]);
+                                mma_f16(o[r][n], va, hi[r][0], hi[r][1]);
+                                mma_f16(o[r][n + 1], vo, hi[r][0], hi[r][1]);
+                                mma_f16(o[r][n], va, lo[r][0], lo[r][1]);
+                                mma_f16(o[r][n + 1], vo, lo[r][0], lo[r][1]);
                             }
                         }
                     }
@@ -681,13 +666,15 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                     for (int e = 0; e < kO; ++e) dst[h * D + lane * kO + e] = of[h][e];
             } else {
                 // [head][fragment row], eights XORed with the head against bank conflicts
+                const float unscale = v_unit > 0.0f ? 1.0f / v_unit : 0.0f;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
                     for (int n = 0; n < kN; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] = o[r][n][e];
+                            dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] =
+                                KV == VELO_KV_INT8 ? o[r][n][e] * unscale : o[r][n][e];
             }
         }
         __syncthreads();
@@ -707,10 +694,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                 const float* src = reinterpret_cast<const float*>(smem + stat_buf[w]) + row * D;
                 const int flip = KV == VELO_KV_F32 ? 0 : (row >> 1 & 3) << 3;
                 float v0, v1;
-                if constexpr (KV == VELO_KV_INT8) {  // dimension gg D / 8 + 2n + half is fragment row 16n + 8 half + gg
-                    const int at = 8 * (d % (D / 8)) + d / (D / 8);
+                if constexpr (KV == VELO_KV_INT8) {  // d even: its tile is even, d + 1 has the same row of the next tile
+                    const int at = (d & ~31) + (d >> 1 & 15);
                     v0 = src[at ^ flip];
-                    v1 = src[(at + 8) ^ flip];
+                    v1 = src[(at + 16) ^ flip];
                 } else {
                     const float2 v = *reinterpret_cast<const float2*>(src + (d ^ flip));
                     v0 = v.x;
