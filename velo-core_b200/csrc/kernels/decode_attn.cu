@@ -89,6 +89,9 @@ __host__ __device__ inline size_t slot_floats(int rows, int D) { return (size_t)
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -133,6 +136,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // Two f32 as a pair of 16-bit parts and the pair of their remainders.
 __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32_t& lo) {
     const __half2 h = __floats2half2_rn(x, y);
@@ -308,16 +317,27 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
             const uint8_t* v0 = static_cast<const uint8_t*>(a.kv.v_pool) + block0 * L::kRow + lane * 16;
             const uint8_t* k1 = static_cast<const uint8_t*>(a.kv.k_pool) + block1 * L::kRow + lane * 16;
             const uint8_t* v1 = static_cast<const uint8_t*>(a.kv.v_pool) + block1 * L::kRow + lane * 16;
-            const bool full = e.w == kFull;
+            auto copy = [&](auto whole) {
 #pragma unroll
-            for (int i = 0; i < kIts; ++i) {
-                const bool second = kTok == 32 && i * kPer >= 16;
-                const uint32_t kd = st + i * 512 + (k_dst ^ (k_swizzle(i * kPer) << 4));
-                const uint32_t vd = st + L::kHalf + i * 512 + (v_dst ^ (v_swizzle(i * kPer) << 4));
-                const int n = full || (e.w >> (i * kPer + lane / kChunks)) & 1 ? 16 : 0;
-                cp_async16(kd, (second ? k1 : k0) + i * 512, n);
-                cp_async16(vd, (second ? v1 : v0) + i * 512, n);
-            }
+                for (int i = 0; i < kIts; ++i) {
+                    const bool second = kTok == 32 && i * kPer >= 16;
+                    const uint32_t kd = st + i * 512 + (k_dst ^ (k_swizzle(i * kPer) << 4));
+                    const uint32_t vd = st + L::kHalf + i * 512 + (v_dst ^ (v_swizzle(i * kPer) << 4));
+                    const uint8_t *ks = (second ? k1 : k0) + i * 512, *vs = (second ? v1 : v0) + i * 512;
+                    if constexpr (decltype(whole)::value) {
+                        cp_async16(kd, ks);
+                        cp_async16(vd, vs);
+                    } else {  // rows past the length are zero-filled
+                        const int n = (e.w >> (i * kPer + lane / kChunks)) & 1 ? 16 : 0;
+                        cp_async16(kd, ks, n);
+                        cp_async16(vd, vs, n);
+                    }
+                }
+            };
+            if (e.w == kFull)
+                copy(std::true_type{});
+            else
+                copy(std::false_type{});
             if (KV == VELO_KV_INT8 && lane < 8) {  // scales: K of both pages, V of both pages
                 const int pg = (lane >> 1) & 1, half = lane & 1;
                 const size_t at = (pg ? block1 + 16 : block0) + half * 8;
@@ -393,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                 constexpr int kT = kTok / 16;
                 float s[kT][R][4];
                 {
-                    float sum[2][kT][R][4] = {};
+                    float sum[2][kT][R][4];
                     if constexpr (KV == VELO_KV_F16) {
                         const int r8 = lane & 7, mi = lane >> 3;
                         const uint32_t kb = st + ((mi & 1) * 8 + r8) * L::kRow;
@@ -402,7 +422,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             uint32_t kf[4];
                             ldmatrix_x4(kf, kb + (((2 * ks + (mi >> 1)) ^ r8) << 4));
 #pragma unroll
-                            for (int r = 0; r < R; ++r) mma_f16(sum[ks & 1][0][r], kf, qb[r][ks][0], qb[r][ks][1]);
+                            for (int r = 0; r < R; ++r) {
+                                if (ks < 2)
+                                    mma_f16_zero(sum[ks][0][r], kf, qb[r][ks][0], qb[r][ks][1]);
+                                else
+                                    mma_f16(sum[ks & 1][0][r], kf, qb[r][ks][0], qb[r][ks][1]);
+                            }
                         }
                     } else {
 #pragma unroll
@@ -424,8 +449,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                                     const uint32_t kf[4] = {even_bytes_f16(w[0][i]), even_bytes_f16(w[1][i]),
                                                             odd_bytes_f16(w[0][i]), odd_bytes_f16(w[1][i])};
 #pragma unroll
-                                    for (int r = 0; r < R; ++r)
-                                        mma_f16(sum[i & 1][kt][r], kf, qb[r][4 * h + i][0], qb[r][4 * h + i][1]);
+                                    for (int r = 0; r < R; ++r) {
+                                        if (h == 0 && i < 2)
+                                            mma_f16_zero(sum[i][kt][r], kf, qb[r][i][0], qb[r][i][1]);
+                                        else
+                                            mma_f16(sum[i & 1][kt][r], kf, qb[r][4 * h + i][0], qb[r][4 * h + i][1]);
+                                    }
                                 }
                             }
                     }
