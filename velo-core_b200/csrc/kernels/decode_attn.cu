@@ -483,53 +483,51 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             s[kt][r][2 * i + 1] *= f;
                         }
                     }
-                if (present != kFull) {
+                // the largest scores and V scale of the step
+                float top[R][2], big = 0.0f;
+                auto largest = [&] {
 #pragma unroll
-                    for (int kt = 0; kt < kT; ++kt)
+                    for (int r = 0; r < R; ++r)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i)
-                            if (!((present >> (kt * 16 + 8 * i + g)) & 1)) {
-                                if constexpr (KV == VELO_KV_INT8) vs[kt][i] = 0.0f;
+                        for (int e = 0; e < 2; ++e) {
+                            float mx = fmaxf(s[0][r][e], s[0][r][2 + e]);
 #pragma unroll
-                                for (int r = 0; r < R; ++r) s[kt][r][2 * i] = s[kt][r][2 * i + 1] = -INFINITY;
-                            }
-                }
-                bool moved = false;
-                if constexpr (KV == VELO_KV_INT8) {
-                    float big = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+                            for (int kt = 1; kt < kT; ++kt) mx = fmaxf(mx, fmaxf(s[kt][r][e], s[kt][r][2 + e]));
 #pragma unroll
-                    for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                    if (big * v_unit > 64.0f || v_unit == 0.0f) {  // the same for the whole warp
+                            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                            top[r][e] = mx;
+                        }
+                    if constexpr (KV == VELO_KV_INT8) {
+                        big = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+                    }
+                };
+                largest();
+                // one rarely taken branch: a ragged step, a new reference, a new unit of the V scales
+                bool adjust = present != kFull || (KV == VELO_KV_INT8 && !(big * v_unit <= 64.0f && v_unit > 0.0f));
+#pragma unroll
+                for (int r = 0; r < R; ++r) adjust |= top[r][0] > m[r][0] + 8.0f || top[r][1] > m[r][1] + 8.0f;
+                if (__any_sync(0xffffffffu, adjust)) {
+                    if (present != kFull) {
+#pragma unroll
+                        for (int kt = 0; kt < kT; ++kt)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                if (!((present >> (kt * 16 + 8 * i + g)) & 1)) {
+                                    if constexpr (KV == VELO_KV_INT8) vs[kt][i] = 0.0f;
+#pragma unroll
+                                    for (int r = 0; r < R; ++r) s[kt][r][2 * i] = s[kt][r][2 * i + 1] = -INFINITY;
+                                }
+                        largest();
+                    }
+                    float f = 1.0f;
+                    if (KV == VELO_KV_INT8 && !(big * v_unit <= 64.0f && v_unit > 0.0f)) {
                         // 2^5 / the power of two below the largest scale (f16: at least 2^-24)
-                        const float unit = big > 0.0f ? __uint_as_float((254u + 5u << 23) - (__float_as_uint(big) & 0x7f800000u)) : 0.0f;
-                        const float f = unit * (v_unit > 0.0f ? 1.0f / v_unit : 0.0f);
+                        const float unit = big > 0.0f ? __uint_as_float(((254u + 5u) << 23) - (__float_as_uint(big) & 0x7f800000u)) : 0.0f;
+                        f = v_unit > 0.0f ? unit / v_unit : 0.0f;
                         v_unit = unit;
-#pragma unroll
-                        for (int r = 0; r < R; ++r)
-#pragma unroll
-                            for (int n = 0; n < kN; ++n)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) o[r][n][e] *= f;
                     }
-#pragma unroll
-                    for (int kt = 0; kt < kT; ++kt)
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) vs[kt][i] *= v_unit;
-                }
-                float top[R][2];
-#pragma unroll
-                for (int r = 0; r < R; ++r)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(s[0][r][e], s[0][r][2 + e]);
-#pragma unroll
-                        for (int kt = 1; kt < kT; ++kt) mx = fmaxf(mx, fmaxf(s[kt][r][e], s[kt][r][2 + e]));
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                        top[r][e] = mx;
-                        moved |= mx > m[r][e] + 8.0f;
-                    }
-                if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -540,10 +538,16 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             l[r][e] *= alpha;
 #pragma unroll
                             for (int n = 0; n < kN; ++n) {
-                                o[r][n][e] *= alpha;
-                                o[r][n][2 + e] *= alpha;
+                                o[r][n][e] *= alpha * f;
+                                o[r][n][2 + e] *= alpha * f;
                             }
                         }
+                }
+                if constexpr (KV == VELO_KV_INT8) {
+#pragma unroll
+                    for (int kt = 0; kt < kT; ++kt)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) vs[kt][i] *= v_unit;
                 }
                 // ---- the weights, as value and remainder, become B fragments by transposition; P V
 #pragma unroll
