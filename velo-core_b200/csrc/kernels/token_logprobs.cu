@@ -10,10 +10,10 @@
 // itself, so the stream needs no barrier.  A thread keeps its own (m, Z, Y)
 // and, per sixteenth of the row, the maximum of what it saw.
 //
-// The n best: the ceil(n / 8)-th largest thread maximum of every warp, least of
-// them over the warps, is a bound that at least n elements reach; only the
-// (thread, sixteenth) pieces whose maximum reaches it are read again (from L2) and
-// their elements at or above it listed -- a few dozen in an ordinary row.  Should
+// The n best: the n-th largest of some of the threads' maxima is a bound that at
+// least n elements reach; only the (thread, sixteenth) pieces whose maximum
+// reaches it are read again and their elements at or above it listed -- little
+// more than n in an ordinary row.  Should
 // the list overflow (ties, ordered rows), it is rebuilt with a higher bound and
 // the ties of the bound are taken in index order.  Positions in the list order
 // decide the rank, so the result does not depend on the order of arrival.
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     constexpr int kN = Vec<T>::n;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums s_part[kWarps];
-    __shared__ uint32_t s_bound[kWarps];
+    __shared__ uint32_t s_bound[kWarps * 32];
     __shared__ int s_count, s_work, s_warp[kWarps];
     __shared__ unsigned long long s_raise;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -350,18 +350,33 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     };
     uint32_t bound = 0;
     if (a.n_top) {
+        // each warp keeps a few more than its share of its threads' maxima; the n-th largest of all
+        // that are kept is a bound which n elements reach
         const int full_warps = min(kWarps, nv / 32);  // warps whose every lane has data
-        const int each = full_warps ? (a.n_top + full_warps - 1) / full_warps : 0;
+        const int keep = full_warps ? min(32, (a.n_top + full_warps - 1) / full_warps + 2) : 0;
+        const int kept = full_warps * keep;
         uint32_t key = order_key(best);
-        for (int i = 0; i < each; ++i) {
-            bound = __reduce_max_sync(0xffffffffu, key);
-            const uint32_t who = __ballot_sync(0xffffffffu, key == bound);
-            if (lane == __ffs(who) - 1) key = 0;
+        for (int i = 0; i < keep; ++i) {
+            const uint32_t top = __reduce_max_sync(0xffffffffu, key);
+            const uint32_t who = __ballot_sync(0xffffffffu, key == top);
+            if (lane == __ffs(who) - 1) {
+                if (warp < full_warps) s_bound[warp * keep + i] = key;
+                key = 0;
+            }
         }
-        if (lane == 0) s_bound[warp] = bound;
         __syncthreads();
-        bound = full_warps ? 0xffffffffu : 0u;
-        for (int i = 0; i < full_warps; ++i) bound = min(bound, s_bound[i]);
+        if (kept >= a.n_top) {
+            for (int i = lane; i < (kept + 31) / 32 * 32; i += 32) {
+                const uint32_t v = i < kept ? s_bound[i] : 0u;
+                int rank = 0;
+                for (int j = 0; j < kept; ++j) rank += s_bound[j] > v || (s_bound[j] == v && j < i);
+                const uint32_t hit = __ballot_sync(0xffffffffu, i < kept && rank == a.n_top - 1);
+                if (hit) {
+                    bound = __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
+                    break;
+                }
+            }
+        }
     } else {
         __syncthreads();
     }
