@@ -34,6 +34,7 @@
 #include <type_traits>
 
 #include "common/elem.cuh"
+#include "common/pdl.cuh"
 #include "common/sm100.cuh"
 #include "common/smem_attr.cuh"
 #include "kernels/decode_ops.h"
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
     constexpr int kTok = L::kTok, S = L::kStages, kRows = 8 * R;
     extern __shared__ __align__(128) uint8_t smem[];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    dependent_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int c = blockIdx.x, Hkv = a.kv.n_kv, Hq = a.Hq;
     const int per_seq = Hkv * plan.tiles;
@@ -770,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
 template <typename Act, int D>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnArgs a, const Plan plan, int rows) {
     __shared__ float wgt[kMaxBlocks], acc[kWarps][D], red[kWarps], red_l[kWarps];
-    asm volatile("griddepcontrol.wait;" ::: "memory");  // the first kernel is complete and visible
+    dependent_wait();  // the first kernel is complete and visible
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int4* desc = static_cast<const int4*>(a.ws);
     const int4 it = desc[c];
@@ -838,21 +839,12 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) 
     const int blocks = p.blocks = std::min(blocks_per_sm(KV, R) * sm_count, kMaxBlocks);
     p.group = a.Hq / a.kv.n_kv;
     p.tiles = (p.group + 8 * R - 1) / (8 * R);
-    decode_attn_kernel<KV, D, R><<<blocks, kThreads, smem, s>>>(a, p);
-    e = cudaGetLastError();
+    e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(blocks), kThreads, smem, 1, s, a, p);
     // no sequence of this table can reach an item that is cut
     if (e != cudaSuccess || (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok <= kWholeUnits) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks, std::min(8 * R, p.group));
-    cfg.blockDim = kThreads;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
-    return cudaLaunchKernelEx(&cfg, decode_join_kernel<Act, D>, a, p, 8 * R);
+    return launch_dependent(decode_join_kernel<Act, D>, dim3(blocks, std::min(8 * R, p.group)), kThreads, 0, 1, s, a, p,
+                            8 * R);
 }
 
 template <int KV, int R>

@@ -10,6 +10,7 @@
 // One block per token: its angles are computed once (a thread per pair) into
 // shared memory, then a thread takes 8 rotation pairs of a head.
 #include "common/elem.cuh"
+#include "common/pdl.cuh"
 #include "kernels/decode_ops.h"
 #include "velo_cuda.h"
 
@@ -39,6 +40,7 @@ template <typename In, typename Act, typename Kv, int D>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs a) {
     constexpr int kLanes = D / 16;  // threads per head, 8 pairs each
     __shared__ float cs[D / 2], sn[D / 2];
+    dependent_wait();
     const int t = blockIdx.x;
     int b = t, first = t;
     if (a.seq_start) {
@@ -139,11 +141,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const KvAppendArgs 
 
 template <typename In, typename Act, typename Kv>
 cudaError_t launch_typed(const KvAppendArgs& a, cudaStream_t s) {
-    if (a.kv.head_dim == 64)
-        kv_append_kernel<In, Act, Kv, 64><<<a.T, kThreads, 0, s>>>(a);
-    else
-        kv_append_kernel<In, Act, Kv, 128><<<a.T, kThreads, 0, s>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(a.kv.head_dim == 64 ? kv_append_kernel<In, Act, Kv, 64> : kv_append_kernel<In, Act, Kv, 128>,
+                            dim3(a.T), kThreads, 0, 1, s, a);
 }
 
 template <typename In>

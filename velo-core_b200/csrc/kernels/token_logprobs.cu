@@ -24,6 +24,7 @@
 #include <type_traits>
 
 #include "common/elem.cuh"
+#include "common/pdl.cuh"
 #include "common/sm100.cuh"
 #include "common/smem_attr.cuh"
 #include "common/spec_math.cuh"
@@ -195,6 +196,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) token_logprobs_kernel(
     __shared__ unsigned long long s_raise;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int cluster = 1 << log_cluster, part = blockIdx.x & (cluster - 1), r = blockIdx.x >> log_cluster;
+    dependent_wait();
     if (cluster > 1) cluster_arrive();  // the first block's inbox may be written once all have started
     const float k = a.inv_t * kLog2e;
     float* slot_max = reinterpret_cast<float*>(smem + kSlotOfs);
@@ -501,18 +503,8 @@ cudaError_t launch_typed(const TokenLogprobsArgs& a, int sm_count, cudaStream_t 
     const int smem = cluster > 1 ? kSmemCluster : kSmemOne;
     cudaError_t e = ensure_smem(attr, token_logprobs_kernel<T>, kSmemCluster);
     if (e != cudaSuccess) return e;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = (unsigned)a.M << log_cluster;
-    cfg.blockDim = kThreads;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cluster;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T>, a, log_cluster);
+    return launch_dependent(token_logprobs_kernel<T>, dim3((unsigned)a.M << log_cluster), kThreads, smem, cluster, s, a,
+                            log_cluster);
 }
 
 }  // namespace
