@@ -160,6 +160,10 @@ __device__ __forceinline__ uint32_t even_bytes_f16(uint32_t w) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 __device__ __forceinline__ uint32_t odd_bytes_f16(uint32_t w) { return even_bytes_f16(w >> 8); }
+// The same bytes plus 128, in units of 2^-24: a byte in a f16's lowest bits is a
+// subnormal the tensor cores multiply exactly, so nothing is subtracted per element.
+__device__ __forceinline__ uint32_t even_bytes_tiny(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t odd_bytes_tiny(uint32_t w) { return even_bytes_tiny(w >> 8); }
 
 // The largest b with pre[b] <= u.
 __device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
@@ -399,6 +403,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                 }
             }
         }
+        // INT8: the scores carry 128 times the sum of q, which comes off each of them (against |q.k|
+        // it is small enough: 128 |sum q| is a few times 127 |q|)
+        float q128[kH][2];
+        if constexpr (KV == VELO_KV_INT8) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&qb[r][ks][i]));
+                        sum += f.x + f.y;
+                    }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);  // head 8r + g
+#pragma unroll
+                for (int e = 0; e < 2; ++e) q128[r][e] = 128.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e));
+            }
+        }
         // INT8: the weights times the V scales are kept within f16 by a power of two that brings
         // the largest scale seen to 2^5 .. 2^6 (0: none yet)
         float v_unit = 0.0f;
@@ -447,8 +471,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                                 }
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const uint32_t kf[4] = {even_bytes_f16(w[0][i]), even_bytes_f16(w[1][i]),
-                                                            odd_bytes_f16(w[0][i]), odd_bytes_f16(w[1][i])};
+                                    const uint32_t kf[4] = {even_bytes_tiny(w[0][i]), even_bytes_tiny(w[1][i]),
+                                                            odd_bytes_tiny(w[0][i]), odd_bytes_tiny(w[1][i])};
 #pragma unroll
                                     for (int r = 0; r < R; ++r) {
                                         if (h == 0 && i < 2)
@@ -479,10 +503,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             vs[kt][i] = lds_half(at + 2 * kTok);
                         }
 #pragma unroll
-                        for (int r = 0; r < R; ++r) {
-                            s[kt][r][2 * i] *= f;
-                            s[kt][r][2 * i + 1] *= f;
-                        }
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float& x = s[kt][r][2 * i + e];
+                                x = (KV == VELO_KV_INT8 ? fmaf(x, 16777216.0f, -q128[r][e]) : x) * f;
+                            }
                     }
                 // the largest scores and V scale of the step
                 float top[R][2], big = 0.0f;
