@@ -58,7 +58,10 @@ constexpr int kRing = 64;  // unit descriptions per warp
 
 // Resident blocks per SM: INT8 pages with at most 8 query heads per KV head need
 // the third (12 warps) to cover the latency of their conversions.
-constexpr int blocks_per_sm(int kv, int R) { return kv == VELO_KV_INT8 && R == 1 ? 3 : 2; }
+constexpr int blocks_per_sm(int kv, int R) { return kv == VELO_KV_INT8 && R <= 1 ? 3 : 2; }
+// Query heads of an item: 8 R, or 4 for R = 0, where the tile's columns 4 .. 7 repeat
+// heads 0 .. 3 and carry the remainders of their weights.
+constexpr int rows_of(int R) { return R ? 8 * R : 4; }
 
 constexpr int tokens_of(int kv) { return kv == VELO_KV_F16 ? 16 : kv == VELO_KV_INT8 ? 32 : 8; }
 constexpr int bytes_of(int kv) { return kv == VELO_KV_F16 ? 2 : kv == VELO_KV_INT8 ? 1 : 4; }
@@ -199,12 +202,14 @@ __device__ __forceinline__ int cut(const int* pre, int B, int per_seq, int total
     return x.units <= max(kWholeUnits, total / blocks / 4) ? x.start : u;
 }
 
-// KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item.
-template <int KV, int D, int R>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_kernel(const DecodeAttnArgs a, const Plan plan) {
-    using L = Layout<KV, D, R>;
+// KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item (0: half a tile).
+template <int KV, int D, int kTiles>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_attn_kernel(const DecodeAttnArgs a,
+                                                                                     const Plan plan) {
+    using L = Layout<KV, D, kTiles>;
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
-    constexpr int kTok = L::kTok, S = L::kStages, kRows = 8 * R;
+    constexpr bool kPair = kTiles == 0;  // columns 4 .. 7 hold remainders
+    constexpr int R = kPair ? 1 : kTiles, kTok = L::kTok, S = L::kStages, kRows = rows_of(kTiles);
     extern __shared__ __align__(128) uint8_t smem[];
     dependent_wait();
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -388,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
         } else {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-                const int row = 8 * r + g;
+                const int row = kPair ? g & 3 : 8 * r + g;
                 const Act* qr = qp + (size_t)row * D;
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
@@ -579,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                 // ---- the weights, as value and remainder, become B fragments by transposition; P V
 #pragma unroll
                 for (int kt = 0; kt < kT; ++kt) {
-                    uint32_t hi[R][2], lo[R][2];
+                    uint32_t hi[R][2], lo[R][2];  // kPair: hi has both
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
@@ -590,8 +595,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             l[r][1] += p1;
                             const float v = KV == VELO_KV_INT8 ? vs[kt][i] : 1.0f;
                             split_f16(p0 * v, p1 * v, hi[r][i], lo[r][i]);
-                            hi[r][i] = transpose8x8(hi[r][i]);
-                            lo[r][i] = transpose8x8(lo[r][i]);
+                            if constexpr (kPair) {
+                                hi[r][i] = transpose8x8(t < 2 ? hi[r][i] : lo[r][i]);
+                            } else {
+                                hi[r][i] = transpose8x8(hi[r][i]);
+                                lo[r][i] = transpose8x8(lo[r][i]);
+                            }
                         }
                     const int r8 = lane & 7, mi = lane >> 3, row = kt * 16 + (mi >> 1) * 8 + r8;
                     const uint32_t vb = st + L::kHalf + row * L::kRow, flip = v_swizzle(row);
@@ -603,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
                                 mma_f16(o[r][n], vf, hi[r][0], hi[r][1]);
-                                mma_f16(o[r][n], vf, lo[r][0], lo[r][1]);
+                                if constexpr (!kPair) mma_f16(o[r][n], vf, lo[r][0], lo[r][1]);
                             }
                         }
                     } else {
@@ -619,8 +628,10 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                             for (int r = 0; r < R; ++r) {
                                 mma_f16(o[r][n], va, hi[r][0], hi[r][1]);
                                 mma_f16(o[r][n + 1], vo, hi[r][0], hi[r][1]);
-                                mma_f16(o[r][n], va, lo[r][0], lo[r][1]);
-                                mma_f16(o[r][n + 1], vo, lo[r][0], lo[r][1]);
+                                if constexpr (!kPair) {
+                                    mma_f16(o[r][n], va, lo[r][0], lo[r][1]);
+                                    mma_f16(o[r][n + 1], vo, lo[r][0], lo[r][1]);
+                                }
                             }
                         }
                     }
@@ -716,6 +727,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                     stat_l[warp * 16 + 8 * r + 2 * t + e] = l[r][e];
                 }
             }
+        if constexpr (kPair && KV != VELO_KV_F32) {  // the remainders' columns join their heads
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[0][n][e] += __shfl_xor_sync(0xffffffffu, o[0][n][e], 2);
+        }
         if (lane == 0) stat_buf[warp] = (int)(buf - smem_u32(smem));
         if (pending) {
             float* dst = reinterpret_cast<float*>(smem + (buf - smem_u32(smem)));
@@ -733,7 +750,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, R)) decode_attn_ke
                     for (int n = 0; n < kN; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] =
+                            if (!kPair || t < 2) dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] =
                                 KV == VELO_KV_INT8 ? o[r][n][e] * unscale : o[r][n][e];
             }
         }
@@ -864,13 +881,13 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) 
     Plan p;
     const int blocks = p.blocks = std::min(blocks_per_sm(KV, R) * sm_count, kMaxBlocks);
     p.group = a.Hq / a.kv.n_kv;
-    p.tiles = (p.group + 8 * R - 1) / (8 * R);
+    p.tiles = (p.group + rows_of(R) - 1) / rows_of(R);
     e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(blocks), kThreads, smem, 1, s, a, p);
     // no sequence of this table can reach an item that is cut
     if (e != cudaSuccess || (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok <= kWholeUnits) return e;
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
-    return launch_dependent(decode_join_kernel<Act, D>, dim3(blocks, std::min(8 * R, p.group)), kThreads, 0, 1, s, a, p,
-                            8 * R);
+    return launch_dependent(decode_join_kernel<Act, D>, dim3(blocks, std::min(rows_of(R), p.group)), kThreads, 0, 1, s, a, p,
+                            rows_of(R));
 }
 
 template <int KV, int R>
@@ -878,23 +895,36 @@ cudaError_t launch_rows(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
     return a.kv.head_dim == 64 ? launch_typed<KV, 64, R>(a, sm_count, s) : launch_typed<KV, 128, R>(a, sm_count, s);
 }
 
-// tiles of 8 query heads per item: f32 items hold 8 heads, the others up to 16
-int row_tiles(int group, int kv_dtype) { return kv_dtype != VELO_KV_F32 && group > 8 ? 2 : 1; }
+// tiles of 8 query heads per item: f32 items hold 8 heads, the others 4 (half the MMAs
+// for P V), 8 or up to 16
+int row_tiles(int group, int kv_dtype) {
+    if (kv_dtype == VELO_KV_F32) return 1;
+    return group > 8 ? 2 : group > 4 ? 1 : 0;
+}
 
 }  // namespace
 
 size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
-    const int R = row_tiles(Hq / Hkv, VELO_KV_INT8);  // the most blocks and the most rows of any page type
-    const size_t blocks = std::min(blocks_per_sm(VELO_KV_INT8, R) * sm_count, kMaxBlocks);
-    return blocks * sizeof(int4) + 2 * blocks * slot_floats(8 * R, D) * sizeof(float);
+    // the most that any page type needs
+    size_t most = 0;
+    for (int kv : {VELO_KV_F16, VELO_KV_INT8, VELO_KV_F32}) {
+        const int R = row_tiles(Hq / Hkv, kv);
+        const size_t blocks = std::min(blocks_per_sm(kv, R) * sm_count, kMaxBlocks);
+        most = std::max(most, blocks * (sizeof(int4) + 2 * slot_floats(rows_of(R), D) * sizeof(float)));
+    }
+    return most;
 }
 
 cudaError_t launch_decode_attention(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
     const int R = row_tiles(a.Hq / a.kv.n_kv, a.kv.kv_dtype);
     if (a.kv.kv_dtype == VELO_KV_F32) return launch_rows<VELO_KV_F32, 1>(a, sm_count, s);
     if (a.kv.kv_dtype == VELO_KV_INT8)
-        return R == 2 ? launch_rows<VELO_KV_INT8, 2>(a, sm_count, s) : launch_rows<VELO_KV_INT8, 1>(a, sm_count, s);
-    return R == 2 ? launch_rows<VELO_KV_F16, 2>(a, sm_count, s) : launch_rows<VELO_KV_F16, 1>(a, sm_count, s);
+        return R == 2   ? launch_rows<VELO_KV_INT8, 2>(a, sm_count, s)
+               : R == 1 ? launch_rows<VELO_KV_INT8, 1>(a, sm_count, s)
+                        : launch_rows<VELO_KV_INT8, 0>(a, sm_count, s);
+    return R == 2   ? launch_rows<VELO_KV_F16, 2>(a, sm_count, s)
+           : R == 1 ? launch_rows<VELO_KV_F16, 1>(a, sm_count, s)
+                    : launch_rows<VELO_KV_F16, 0>(a, sm_count, s);
 }
 
 }  // namespace velo
