@@ -44,26 +44,47 @@ def test_turn_fractions_keep_far_angles(base, D):
             assert min(off, 2 - off) <= 2.0 ** -23
 
 
-def _ranges(units, per_seq, blocks, whole=16, least=4):
+class _Share:
+    """n units in k ranges, the first n % k with one more (decode_attn.cu)."""
+
+    def __init__(self, n, k):
+        self.n, self.k, self.q, self.r = n, k, n // k if k else 0, n % k if k else 0
+
+    def at(self, c):
+        return c * self.q + min(c, self.r)
+
+    def range_of(self, u):
+        head = self.r * (self.q + 1)
+        return u // (self.q + 1) if u < head else self.r + (u - head) // self.q
+
+
+def _ranges(units, per_seq, main, tail, whole=16, least=4, share=12, tail_units=64, tail_states=24):
     """decode_attn.cu's cut of the unit list: per block its pieces (item, first,
-    last + 1 unit of the item), the slot of each partial piece, and the open
-    item's last block."""
+    last + 1 unit of the item, units, slot of a partial piece), and the open item
+    with its last block."""
     pre = np.concatenate(([0], np.cumsum(np.asarray(units) * per_seq)))
     total = int(pre[-1])
-    blocks = min(blocks, -(-total // least))
+    if tail and total // main >= tail_units and max(units) <= tail_states * (total // share // tail):
+        big, small = _Share(total - total // share, main), _Share(total // share, tail)
+    else:
+        big, small = _Share(total, min(main, -(-total // least))), _Share(0, 0)
+    blocks = big.k + small.k
 
     def item(u):
         b = int(np.searchsorted(pre, u, "right")) - 1
-        n = int(pre[b + 1] - pre[b]) // per_seq
+        n = int(units[b])
         it = int(u - pre[b]) // n
         return (b, it), int(pre[b]) + it * n, n
 
     def cut(c):
-        u = total * c // blocks
+        u = total if c >= blocks else big.at(c) if c <= big.k else big.n + small.at(c - big.k)
         if c == 0 or u >= total:
             return u
         _, start, n = item(u)
-        return start if n <= max(whole, total // blocks // 4) else u
+        return start if n <= max(whole, (big.q if c <= big.k else small.q) // 4) else u
+
+    def block_of(u):
+        return big.range_of(u) if u < big.n else big.k + small.range_of(u - big.n)
     out = []
     for c in range(blocks):
         seg, u1 = cut(c), cut(c + 1)
@@ -75,24 +96,24 @@ def _ranges(units, per_seq, blocks, whole=16, least=4):
             pieces.append((key, seg - start, stop - start, n, None if full else 2 * c + (seg == start)))
             if not full and seg == start:
                 assert open_ is None
-                open_ = (key, (end * blocks - 1) // total)
+                open_ = (key, block_of(end - 1))
             seg = stop
         out.append((pieces, open_))
     return out
 
 
-@pytest.mark.parametrize("seed", range(40))
+@pytest.mark.parametrize("seed", range(60))
 def test_decode_work_list_covers_every_item_once(seed):
     """Every unit of every item is in exactly one block; an item cut between
     blocks is open in its first one, whose join reads slot 1 of that block and
     slot 0 of the following ones, each written once."""
     rng = np.random.default_rng(seed)
     B = int(rng.integers(1, 30))
-    units = rng.integers(0, int(rng.choice([2, 20, 500])), B)
+    units = rng.integers(0, int(rng.choice([2, 20, 500, 3000])), B)
     if not units.any():
         units[0] = 1
-    per_seq, blocks = int(rng.choice([1, 2, 8, 32])), int(rng.choice([1, 7, 296]))
-    out = _ranges(units, per_seq, blocks)
+    per_seq, main = int(rng.choice([1, 2, 8, 32])), int(rng.choice([1, 7, 296]))
+    out = _ranges(units, per_seq, main, main * int(rng.choice([0, 1, 2])))
     got, written = {}, {}
     for pieces, _ in out:
         for key, lo, hi, n, slot in pieces:

@@ -8,11 +8,11 @@
 // Work: the batch is one list of units -- a unit is a step of 16 (f16), 32 (int8)
 // or 8 (f32) tokens of one item, an item a (sequence, KV head, tile of query
 // heads) -- cut into equal ranges, one per block, two blocks per SM, whatever the
-// lengths are.  An item that a cut runs through leaves partial states (max, sum,
-// unnormalised output) in the workspace, which the join kernel, launched as a
-// programmatic dependent, adds in order: no atomics, repeatable bits.  Short
-// items are not cut (the cut moves to their start), so a batch of short contexts
-// pays no join.
+// lengths are (and a tail of short ranges, for balance).  An item that a cut runs
+// through leaves partial states (max, sum, unnormalised output) in the workspace,
+// which the join kernel, launched as a programmatic dependent, adds in order: no
+// atomics, repeatable bits.  Short items are not cut (the cut moves to their
+// start), so a batch of short contexts pays no join.
 //
 // A block's four warps take the units of its range in turn.  Each warp streams
 // its own units through a private ring of 8 KB (head_dim 128) stages filled by
@@ -49,7 +49,6 @@ using sm100::smem_u32;
 constexpr int kErrSeqLen = 0x6211, kErrPage = 0x6212;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kMaxBlocks = 1024;
 constexpr int kMinUnits = 4;  // units per block at least: one per warp
 // An item of at most this many units (256 tokens of f16 pages), or of a quarter of
 // a block's range, is never cut.
@@ -82,7 +81,7 @@ struct Layout {
 };
 
 struct Plan {
-    int blocks;   // of the grid
+    int main, blocks;  // resident blocks; with the tail's, the grid
     int group;    // query heads per KV head
     int tiles;    // query-head tiles per KV head
 };
@@ -184,22 +183,61 @@ __device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
 struct Item {
     int b, it, start, units;  // sequence, item of the sequence, first unit, units
 };
-__device__ __forceinline__ Item item_of(const int* pre, int B, int per_seq, int u) {
+template <int kTok>
+__device__ __forceinline__ Item item_of(const int* pre, const int* lens, int B, int u) {
     Item x;
     x.b = find_sequence(pre, B, u);
-    x.units = (pre[x.b + 1] - pre[x.b]) / per_seq;
+    x.units = (lens[x.b] + kTok - 1) / kTok;
     x.it = (u - pre[x.b]) / x.units;
     x.start = pre[x.b] + x.it * x.units;
     return x;
 }
 
-// First unit of block c: an equal share of the list, moved to the start of the
-// item it falls into when that item is short.
-__device__ __forceinline__ int cut(const int* pre, int B, int per_seq, int total, int blocks, int c) {
-    const int u = (int)((long long)total * c / blocks);
-    if (c == 0 || u >= total) return u;
-    const Item x = item_of(pre, B, per_seq, u);
-    return x.units <= max(kWholeUnits, total / blocks / 4) ? x.start : u;
+// The cut of the list.  `main` blocks, resident from the start, have equal ranges.
+// SMs do not advance alike (range ends of one launch were 30 % apart), so when a
+// range is long the last twelfth of the list is left to short ranges in
+// blocks that start as the first ones end (ragged INT8 batch of 128: 227 -> 207 us at
+// full clock, 236 -> 234 under the power cap; 64 x 4096 f16: 173.7 -> 171).
+constexpr int kTailPerMain = 1, kTailShare = 12;  // blocks; part of the list
+constexpr int kTailUnits = 64;                   // least large range
+constexpr int kTailStates = 24;                  // most short ranges of an item: its join reads that many states
+// n units in k ranges: the first n % k have one unit more.
+struct Share {
+    int n, k, q, r;
+    __device__ __forceinline__ Share(int n_, int k_) : n(n_), k(k_), q(k_ ? n_ / k_ : 0), r(n_ - q * k_) {}
+    __device__ __forceinline__ int at(int c) const { return c * q + min(c, r); }  // first unit of range c
+    __device__ __forceinline__ int range_of(int u) const {
+        return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q;
+    }
+};
+struct Cut {
+    Share big, tail;  // the large ranges, then the short ones
+    __device__ __forceinline__ int blocks() const { return big.k + tail.k; }
+    __device__ __forceinline__ int total() const { return big.n + tail.n; }
+    __device__ __forceinline__ int at(int c) const { return c <= big.k ? big.at(c) : big.n + tail.at(c - big.k); }
+    __device__ __forceinline__ int block_of(int u) const {
+        return u < big.n ? big.range_of(u) : big.k + tail.range_of(u - big.n);
+    }
+    // Items up to this length are not cut by the start of block c (never more in the tail, so
+    // that moving a cut to an item's start keeps the cuts in order).
+    __device__ __forceinline__ int whole(int c) const { return max(kWholeUnits, (c <= big.k ? big.q : tail.q) / 4); }
+};
+__device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int longest) {
+    const int tail = plan.blocks - plan.main;
+    if (tail > 0 && total / plan.main >= kTailUnits && longest <= kTailStates * (total / kTailShare / tail)) {
+        const int n = total / kTailShare;
+        return Cut{Share(total - n, plan.main), Share(n, tail)};
+    }
+    return Cut{Share(total, min(plan.main, (total + kMinUnits - 1) / kMinUnits)), Share(0, 0)};
+}
+
+// First unit of block c: moved to the start of the item it falls into when that is short.
+template <int kTok>
+__device__ __forceinline__ int cut_at(const int* pre, const int* lens, int B, const Cut& k, int c) {
+    const int u = c < k.blocks() ? k.at(c) : k.total();
+    if (c == 0 || u >= k.total()) return u;
+    const Item x = item_of<kTok>(pre, lens, B, u);
+    return x.units <= k.whole(c) ? x.start : u;
 }
 
 // KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item (0: half a tile).
@@ -220,14 +258,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
     int* stat_buf = reinterpret_cast<int*>(stat_l + kWarps * 16);
     int* lens = reinterpret_cast<int*>(smem + L::kLens);
     int* pre = lens + a.B;
-    __shared__ int s_warp[kWarps], s_cut[2];
+    __shared__ int s_warp[kWarps], s_long[kWarps], s_cut[2];
     int4* desc = static_cast<int4*>(a.ws);
     float* slots = reinterpret_cast<float*>(desc + plan.blocks);
 
     // lengths and units before each sequence
     {
         const int per = (a.B + kThreads - 1) / kThreads, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
-        int sum = 0;
+        int sum = 0, longest = 0;
         for (int b = lo; b < hi; ++b) {
             int n = a.seq_len[b];
             if (n < 0 || n > a.kv.max_pages * kPageTokens) {
@@ -237,6 +275,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
             lens[b] = n;
             pre[b] = sum;
             sum += (n + kTok - 1) / kTok * per_seq;
+            longest = max(longest, (n + kTok - 1) / kTok);
         }
         int x = sum;
 #pragma unroll
@@ -244,7 +283,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        if (lane == 31) s_warp[warp] = x;
+        if (plan.blocks > plan.main) longest = __reduce_max_sync(0xffffffffu, longest);
+        if (lane == 31) {
+            s_warp[warp] = x;
+            s_long[warp] = longest;
+        }
         __syncthreads();
         int before = x - sum;
         for (int w = 0; w < warp; ++w) before += s_warp[w];
@@ -253,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         __syncthreads();
     }
     const int total = pre[a.B];
-    const int blocks = min(plan.blocks, (total + kMinUnits - 1) / kMinUnits);
+    const Cut list = cut_list(plan, total, max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3])));
 
     // sequences without tokens
     for (int b = c; b < a.B; b += gridDim.x) {
@@ -262,11 +305,11 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         if (a.lse)
             for (int i = tid; i < Hq; i += kThreads) a.lse[(size_t)b * Hq + i] = -INFINITY;
     }
-    if (c >= blocks) {
+    if (c >= list.blocks()) {
         if (tid == 0) desc[c] = make_int4(-1, 0, 0, 0);
         return;
     }
-    if (tid < 2) s_cut[tid] = cut(pre, a.B, per_seq, total, blocks, c + tid);
+    if (tid < 2) s_cut[tid] = cut_at<kTok>(pre, lens, a.B, list, c + tid);
     __syncthreads();
     const int u0 = s_cut[0], u1 = s_cut[1];
 
@@ -278,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         const int j = j0 + lane;
         if (j >= n_w) return;
         const int u = u0 + warp + kWarps * j;
-        const Item x = item_of(pre, a.B, per_seq, u);
+        const Item x = item_of<kTok>(pre, lens, a.B, u);
         const int first = (u - x.start) * kTok, left = lens[x.b] - first;
         const uint32_t* row = a.kv.page_table + (size_t)x.b * a.kv.max_pages + first / kPageTokens;
         uint4 e = make_uint4(row[0], 0, (uint32_t)(x.it / plan.tiles), left >= 32 ? ~0u : (1u << left) - 1);
@@ -363,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
     int j = 0;
     int4 open = make_int4(-1, 0, 0, 0);
     for (int seg = u0; seg < u1;) {
-        const Item x = item_of(pre, a.B, per_seq, seg);
+        const Item x = item_of<kTok>(pre, lens, a.B, seg);
         const int end = x.start + x.units, seg_end = min(end, u1);
         const int hk = x.it / plan.tiles, tile = x.it % plan.tiles;
         const int h0 = hk * plan.group + tile * kRows, nh = min(kRows, plan.group - tile * kRows);
@@ -801,7 +844,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         __syncthreads();
         if (pending) issue(j - 1 + S);
         if (!whole && seg == x.start)  // begins here, ends in a later block
-            open = make_int4(x.b, x.it, (int)(((long long)end * blocks - 1) / total), 0);
+            open = make_int4(x.b, x.it, list.block_of(end - 1), 0);
         seg = seg_end;
     }
     cp_async_wait<0>();
@@ -810,10 +853,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
 
 // Joins the partial states of the item that block x of the first kernel left
 // open: slot 1 of that block, slot 0 of the following ones.  One block per (open
-// item, query head); a warp adds every fourth state.
+// item, query head); each of its warps takes every fourth state, eight at a time
+// (maxima, sums and outputs in one round of reads, the running maximum as in the
+// first kernel), and the four results are added in order.
 template <typename Act, int D>
 __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnArgs a, const Plan plan, int rows) {
-    __shared__ float wgt[kMaxBlocks], acc[kWarps][D], red[kWarps], red_l[kWarps];
+    __shared__ float acc[kWarps][D], s_m[kWarps], s_l[kWarps];
     dependent_wait();  // the first kernel is complete and visible
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int4* desc = static_cast<const int4*>(a.ws);
@@ -822,54 +867,75 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnA
     const int hk = it.y / plan.tiles, tile = it.y % plan.tiles;
     if (tile * rows + row >= plan.group) return;
     const int head = hk * plan.group + tile * rows + row;
-    const float* slots = reinterpret_cast<const float*>(desc + plan.blocks);
     const size_t step = slot_floats(rows, D);
+    const float* first = reinterpret_cast<const float*>(desc + plan.blocks) + (size_t)(2 * c) * step;
     const int n = it.z - c + 1;
-    auto state = [&](int i) { return slots + (size_t)(i == 0 ? 2 * c + 1 : 2 * (c + i)) * step; };
-    float M = -INFINITY;
-    for (int i = tid; i < n; i += kThreads) {
-        const float mi = state(i)[2 * row];
-        wgt[i] = mi;
-        M = fmaxf(M, mi);
-    }
+    constexpr int kE = D / 32, kBatch = 8;
+    float m = -INFINITY, l = 0.0f, x[kE] = {};
+    for (int i0 = warp; i0 < n; i0 += kWarps * kBatch) {
+        float2 ml[kBatch];
+        float o[kBatch][kE];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
+        for (int j = 0; j < kBatch; ++j) {
+            const int i = i0 + j * kWarps;
+            ml[j] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red[w]);
-    float Ls = 0.0f;
-    for (int i = tid; i < n; i += kThreads) {
-        const float li = state(i)[2 * row + 1];
-        const float f = li == 0.0f ? 0.0f : ex2_approx(wgt[i] - M);
-        wgt[i] = f;
-        Ls += li * f;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) Ls += __shfl_xor_sync(0xffffffffu, Ls, o);
-    if (lane == 0) red_l[warp] = Ls;
-    __syncthreads();
-    Ls = red_l[0] + red_l[1] + red_l[2] + red_l[3];
-    constexpr int kE = D / 32;
-    float x[kE] = {};
-#pragma unroll 8
-    for (int i = warp; i < n; i += kWarps) {
-        const float f = wgt[i];
-        const float* p = state(i) + 2 * rows + row * D + lane * kE;
-        if (f != 0.0f) {
-#pragma unroll
-            for (int e = 0; e < kE; ++e) x[e] = fmaf(p[e], f, x[e]);
+            for (int e = 0; e < kE; ++e) o[j][e] = 0.0f;
+            if (i < n) {
+                const float* st = first + (i == 0 ? 1 : 2 * (size_t)i) * step;
+                ml[j] = *reinterpret_cast<const float2*>(st + 2 * row);
+                const float* p = st + 2 * rows + row * D + lane * kE;
+                if constexpr (kE == 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(p);
+                    o[j][0] = v.x, o[j][1] = v.y, o[j][2] = v.z, o[j][3] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(p);
+                    o[j][0] = v.x, o[j][1] = v.y;
+                }
+            }
         }
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) top = fmaxf(top, ml[j].x);
+        const float ref = top == -INFINITY ? 0.0f : top, alpha = ex2_approx(m - ref);
+        m = top;
+        l *= alpha;
+#pragma unroll
+        for (int e = 0; e < kE; ++e) x[e] *= alpha;
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const float f = ex2_approx(ml[j].x - ref);
+            l = fmaf(ml[j].y, f, l);
+#pragma unroll
+            for (int e = 0; e < kE; ++e) x[e] = fmaf(o[j][e], f, x[e]);
+        }
+    }
+    if (lane == 0) {
+        s_m[warp] = m;
+        s_l[warp] = l;
     }
 #pragma unroll
     for (int e = 0; e < kE; ++e) acc[warp][lane * kE + e] = x[e];
     __syncthreads();
-    const float inv = Ls == 0.0f ? 0.0f : 1.0f / Ls;
+    float M = -INFINITY, L = 0.0f, f[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        f[w] = ex2_approx(s_m[w] - (M == -INFINITY ? 0.0f : M));
+        L = fmaf(s_l[w], f[w], L);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     for (int d = tid; d < D; d += kThreads)
         static_cast<Act*>(a.out)[((size_t)it.x * a.Hq + head) * D + d] =
-            (Act)((acc[0][d] + acc[1][d] + acc[2][d] + acc[3][d]) * inv);
-    if (tid == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = Ls == 0.0f ? -INFINITY : (M + log2f(Ls)) * kLn2;
+            (Act)((acc[0][d] * f[0] + acc[1][d] * f[1] + acc[2][d] * f[2] + acc[3][d] * f[3]) * inv);
+    if (tid == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
+
+int main_blocks(int kv, int R, int sm_count) {
+    return blocks_per_sm(kv, R) * sm_count;
+}
+int all_blocks(int kv, int R, int sm_count) { return main_blocks(kv, R, sm_count) * (1 + kTailPerMain); }
 
 template <int KV, int D, int R>
 cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
@@ -879,15 +945,22 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) 
     cudaError_t e = ensure_smem(attr, decode_attn_kernel<KV, D, R>, smem);
     if (e != cudaSuccess) return e;
     Plan p;
-    const int blocks = p.blocks = std::min(blocks_per_sm(KV, R) * sm_count, kMaxBlocks);
+    p.main = main_blocks(KV, R, sm_count);
+    p.blocks = all_blocks(KV, R, sm_count);
     p.group = a.Hq / a.kv.n_kv;
     p.tiles = (p.group + rows_of(R) - 1) / rows_of(R);
-    e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(blocks), kThreads, smem, 1, s, a, p);
-    // no sequence of this table can reach an item that is cut
-    if (e != cudaSuccess || (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok <= kWholeUnits) return e;
+    // the tail's blocks only where cut_list can come to use them: enough work in this table,
+    // and enough items that the longest is not above kTailStates short ranges
+    const int most = (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok;  // units of an item at most
+    const long long items = (long long)a.B * a.kv.n_kv * p.tiles;
+    if (items * most < (long long)kTailUnits * p.main ||
+        items * kTailStates < (long long)kTailShare * (p.blocks - p.main))
+        p.blocks = p.main;
+    e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(p.blocks), kThreads, smem, 1, s, a, p);
+    if (e != cudaSuccess || most <= kWholeUnits) return e;  // no item of this table is ever cut
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
-    return launch_dependent(decode_join_kernel<Act, D>, dim3(blocks, std::min(rows_of(R), p.group)), kThreads, 0, 1, s, a, p,
-                            rows_of(R));
+    return launch_dependent(decode_join_kernel<Act, D>, dim3(p.blocks, std::min(rows_of(R), p.group)), kThreads, 0, 1, s, a,
+                            p, rows_of(R));
 }
 
 template <int KV, int R>
@@ -909,7 +982,7 @@ size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
     size_t most = 0;
     for (int kv : {VELO_KV_F16, VELO_KV_INT8, VELO_KV_F32}) {
         const int R = row_tiles(Hq / Hkv, kv);
-        const size_t blocks = std::min(blocks_per_sm(kv, R) * sm_count, kMaxBlocks);
+        const size_t blocks = all_blocks(kv, R, sm_count);
         most = std::max(most, blocks * (sizeof(int4) + 2 * slot_floats(rows_of(R), D) * sizeof(float)));
     }
     return most;
