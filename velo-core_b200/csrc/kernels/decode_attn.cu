@@ -153,19 +153,11 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
     hi = *reinterpret_cast<const uint32_t*>(&h);
     lo = *reinterpret_cast<const uint32_t*>(&r);
 }
-// The even (odd) bytes of w, int8, as an exact f16 pair: 0x6400 | u is 1024 + u,
-// u = the byte with its sign bit flipped, and 1152 comes off again.
-__device__ __forceinline__ uint32_t even_bytes_f16(uint32_t w) {
-    uint32_t v = (w & 0x00ff00ffu) ^ 0x64806480u;
-    const uint32_t bias = 0x64806480u;
-    const __half2 r = __hsub2(*reinterpret_cast<__half2*>(&v), *reinterpret_cast<const __half2*>(&bias));
-    return *reinterpret_cast<const uint32_t*>(&r);
-}
-__device__ __forceinline__ uint32_t odd_bytes_f16(uint32_t w) { return even_bytes_f16(w >> 8); }
-// The same bytes plus 128, in units of 2^-24: a byte in a f16's lowest bits is a
-// subnormal the tensor cores multiply exactly, so nothing is subtracted per element.
-__device__ __forceinline__ uint32_t even_bytes_tiny(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
-__device__ __forceinline__ uint32_t odd_bytes_tiny(uint32_t w) { return even_bytes_tiny(w >> 8); }
+// The even (odd) bytes of w, int8, plus 128 and in units of 2^-24, as an f16 pair: a
+// byte in the lowest bits of a f16 is a subnormal, which the tensor cores multiply
+// exactly.  The 128 comes off the sums instead of every element.
+__device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
+__device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return even_bytes(w >> 8); }
 
 // The largest b with pre[b] <= u.
 __device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
@@ -519,8 +511,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                                 }
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) {
-                                    const uint32_t kf[4] = {even_bytes_tiny(w[0][i]), even_bytes_tiny(w[1][i]),
-                                                            odd_bytes_tiny(w[0][i]), odd_bytes_tiny(w[1][i])};
+                                    const uint32_t kf[4] = {even_bytes(w[0][i]), even_bytes(w[1][i]),
+                                                            odd_bytes(w[0][i]), odd_bytes(w[1][i])};
 #pragma unroll
                                     for (int r = 0; r < R; ++r) {
                                         if (h == 0 && i < 2)
@@ -625,6 +617,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                         for (int i = 0; i < 2; ++i) vs[kt][i] *= v_unit;
                 }
                 // ---- the weights, as value and remainder, become B fragments by transposition; P V
+                float bias[R][4];
 #pragma unroll
                 for (int kt = 0; kt < kT; ++kt) {
                     uint32_t hi[R][2], lo[R][2];  // kPair: hi has both
@@ -659,14 +652,26 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                             }
                         }
                     } else {
+                        // minus 128 times the weights, as the same products: what the step's outputs carry too much
+                        const uint32_t minus128[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            if (kt == 0)
+                                mma_f16_zero(bias[r], minus128, hi[r][0], hi[r][1]);
+                            else
+                                mma_f16(bias[r], minus128, hi[r][0], hi[r][1]);
+                            if constexpr (!kPair) mma_f16(bias[r], minus128, lo[r][0], lo[r][1]);
+                        }
                         // transposed as 16-bit units, a register holds two dimensions of two tokens:
                         // row 8 half + g of tile n is dimension 32 (n / 2) + 16 half + 2 g + n % 2
 #pragma unroll
                         for (int n = 0; n < kN; n += 2) {
                             uint32_t w[4];
                             ldmatrix_x4_trans(w, vb + (((n + (mi & 1)) ^ flip) << 4));
-                            const uint32_t va[4] = {even_bytes_f16(w[0]), even_bytes_f16(w[1]), even_bytes_f16(w[2]), even_bytes_f16(w[3])};
-                            const uint32_t vo[4] = {odd_bytes_f16(w[0]), odd_bytes_f16(w[1]), odd_bytes_f16(w[2]), odd_bytes_f16(w[3])};
+                            const uint32_t va[4] = {even_bytes(w[0]), even_bytes(w[1]), even_bytes(w[2]),
+                                                    even_bytes(w[3])};
+                            const uint32_t vo[4] = {odd_bytes(w[0]), odd_bytes(w[1]), odd_bytes(w[2]),
+                                                    odd_bytes(w[3])};
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
                                 mma_f16(o[r][n], va, hi[r][0], hi[r][1]);
@@ -678,6 +683,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                             }
                         }
                     }
+                }
+                if constexpr (KV == VELO_KV_INT8) {
+                    // taken off after every step, the bias never outgrows a step's own weights in the sums
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int n = 0; n < kN; ++n)
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2) {
+                                const float2 x = __fadd2_rn(make_float2(o[r][n][e], o[r][n][e + 1]), make_float2(bias[r][0], bias[r][1]));
+                                o[r][n][e] = x.x;
+                                o[r][n][e + 1] = x.y;
+                            }
                 }
             } else {
                 // ---- f32 scores: token g, dimensions 16 i + 4 t .. + 3 of every head
@@ -786,7 +804,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                     for (int e = 0; e < kO; ++e) dst[h * D + lane * kO + e] = of[h][e];
             } else {
                 // [head][fragment row], eights XORed with the head against bank conflicts
-                const float unscale = v_unit > 0.0f ? 1.0f / v_unit : 0.0f;
+                const float unscale = v_unit > 0.0f ? 16777216.0f / v_unit : 0.0f;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
