@@ -301,37 +301,41 @@ typedef struct velo_kv_cache {
     int32_t pool_pages, max_pages, n_kv, head_dim;
 } velo_kv_cache;
 
+/* The new tokens of velo_cuda_kv_append (all pointers device memory). */
+typedef struct velo_kv_append_batch {
+    uint32_t struct_size;     /* sizeof(velo_kv_append_batch) */
+    int32_t in_dtype;         /* velo_elem of q, k and v */
+    const void *q;            /* [n_tokens][n_head][head_dim] (or NULL with q_out NULL, n_head 0) */
+    const void *k, *v;        /* [n_tokens][n_kv][head_dim] */
+    int64_t ldq, ldk, ldv;    /* token t's row starts at t * ld elements, so that all three may be
+                                 slices of one projection's output; rows 16-byte aligned */
+    const int32_t *seq_start; /* [B+1], non-decreasing: tokens seq_start[b] .. seq_start[b+1] - 1
+                                 continue sequence b; rows from seq_start[B] on are padding, for
+                                 which nothing is read or written.  NULL: token t is sequence t's
+                                 only one (n_tokens == B) */
+    const int32_t *ctx_len;   /* [B] tokens cached before the call: token t of sequence b goes to
+                                 position ctx_len[b] + t - seq_start[b] */
+    int32_t B, n_tokens, n_head;
+    float freq_base;          /* RoPE base, above 1 */
+    void *q_out;              /* [n_tokens][n_head][head_dim], f32 for f32 pages, else f16 */
+    void *k_out, *v_out;      /* [n_tokens][n_kv][head_dim] of q_out's type, or both NULL: the rows as
+                                 the cache now holds them (INT8: q * scale), for attention among
+                                 the new tokens (node_k / node_v of velo_cuda_tree_attention) */
+} velo_kv_append_batch;
+
 /* Append the K/V rows of new tokens to the cache, rotated to their positions on
  * the way, and rotate their queries (RoPE of the verify step: NeoX half split,
  * llama_cpu.rs:98-132; the angles are reduced exactly, so far positions keep
- * their precision).  Device memory, asynchronous on the context stream.
- *   q [n_tokens][n_head][head_dim], k and v [n_tokens][n_kv][head_dim]: elements
- *             of in_dtype (velo_elem); token t's row starts at t * ldq / ldk /
- *             ldv elements, so all three may be slices of one projection's
- *             output.  Rows 16-byte aligned.  Without q: q and q_out NULL, n_head 0.
- *   seq_start [B+1] i32, non-decreasing: tokens seq_start[b] ..
- *             seq_start[b+1] - 1 continue sequence b; rows from seq_start[B] on
- *             are padding (nothing is read or written for them).  NULL: token t
- *             is sequence t's only one (n_tokens == B).
- *   ctx_len   [B] i32 tokens cached before the call: token t of sequence b goes
- *             to position ctx_len[b] + t - seq_start[b].
- *   q_out     [n_tokens][n_head][head_dim], f32 for f32 pages, else f16
- *   k_out, v_out  [n_tokens][n_kv][head_dim] (type of q_out; both or NULL): the rows
- *             as the cache now holds them (INT8: q * scale), for attention
- *             among the new tokens (node_k / node_v of velo_cuda_tree_attention)
- * f16 and f32 pages take the rotated value rounded once; INT8 pages quantise it
- * as velo_cuda_write_kv does (scale = f16(max|x| / 127), truncation).  A
- * position past the page-table row, a page id outside the pool or a negative
- * ctx_len sets the device flag (velo_cuda_sync); that token's K/V are not
- * written.  Page-table rows must not share the pages written here.  Replaces
- * kv_update / kv_update_int8 (src/kernels.metal:619-645, 753-802) after the
- * per-head rope of forward_one (src/llama_cpu.rs:113-132). */
-VELO_API int32_t velo_cuda_kv_append(velo_cuda_ctx *ctx, const velo_kv_cache *cache, const void *q,
-                                     const void *k, const void *v, int32_t in_dtype, int64_t ldq,
-                                     int64_t ldk, int64_t ldv, const int32_t *seq_start,
-                                     const int32_t *ctx_len, int32_t B, int32_t n_tokens,
-                                     int32_t n_head, float freq_base, void *q_out, void *k_out,
-                                     void *v_out);
+ * their precision).  Asynchronous on the context stream.  f16 and f32 pages take
+ * the rotated value rounded once; INT8 pages quantise it as velo_cuda_write_kv
+ * does (scale = f16(max|x| / 127), truncation).  A position past the page-table
+ * row, a page id outside the pool or a negative ctx_len sets the device flag
+ * (velo_cuda_sync); that token's K/V are not written.  Page-table rows must not
+ * share the pages written here.  Replaces kv_update / kv_update_int8
+ * (src/kernels.metal:619-645, 753-802) after the per-head rope of forward_one
+ * (src/llama_cpu.rs:113-132). */
+VELO_API int32_t velo_cuda_kv_append(velo_cuda_ctx *ctx, const velo_kv_cache *cache,
+                                     const velo_kv_append_batch *batch);
 
 /* Device bytes of the workspace velo_cuda_decode_attention needs (any B and any
  * lengths) for these head counts; 0 for arguments that call refuses. */

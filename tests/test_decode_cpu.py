@@ -9,7 +9,7 @@ import velo_cuda
 def test_null_context_is_refused():
     L = velo_cuda.lib()
     bad = velo_cuda.ERR_INVALID_ARGUMENT
-    assert L.velo_cuda_kv_append(None, None, None, None, None, 0, 0, 0, 0, None, None, 1, 1, 1, 1e4, None, None, None) == bad
+    assert L.velo_cuda_kv_append(None, None, None) == bad
     assert "NULL" in velo_cuda.last_error()
     assert L.velo_cuda_decode_attention(None, None, None, 0, None, 1, 1, 0.0, None, None, None, 0) == bad
     assert L.velo_cuda_token_logprobs(None, None, 0, 1, 1, 1, None, 1.0, None, None, 0, None, None) == bad

@@ -81,56 +81,59 @@ const velo::RopeTurns& rope_turns(velo_cuda_ctx* c, float base, int D) {
 
 extern "C" {
 
-int32_t velo_cuda_kv_append(velo_cuda_ctx* c, const velo_kv_cache* cache, const void* q, const void* k,
-                            const void* v, int32_t in_dtype, int64_t ldq, int64_t ldk, int64_t ldv,
-                            const int32_t* seq_start, const int32_t* ctx_len, int32_t B, int32_t n_tokens,
-                            int32_t n_head, float freq_base, void* q_out, void* k_out, void* v_out) {
+int32_t velo_cuda_kv_append(velo_cuda_ctx* c, const velo_kv_cache* cache, const velo_kv_append_batch* in) {
     velo::Range nvtx_range("velo.kv_append");
     velo::clear_last_error();
     if (!c) return fail(VELO_ERR_INVALID_ARGUMENT, "ctx is NULL");
     velo::KvAppendArgs a{};
     int32_t st = check_cache("kv_append", cache, a.kv);
     if (st) return st;
-    if (in_dtype < VELO_ELEM_F32 || in_dtype > VELO_ELEM_BF16)
-        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: in_dtype %d", in_dtype);
-    if (n_head != 0 && bad_heads(n_head, cache->n_kv))
-        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: n_head %d / n_kv %d", n_head, cache->n_kv);
-    if (!(freq_base > 1.0f) || std::isinf(freq_base))
+    if (!in) return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: batch is NULL");
+    if (in->struct_size != sizeof(velo_kv_append_batch))
+        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: velo_kv_append_batch.struct_size %u != %zu", in->struct_size,
+                    sizeof(velo_kv_append_batch));
+    const int D = cache->head_dim, n_kv = cache->n_kv;
+    if (in->in_dtype < VELO_ELEM_F32 || in->in_dtype > VELO_ELEM_BF16)
+        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: in_dtype %d", in->in_dtype);
+    if (in->n_head != 0 && bad_heads(in->n_head, n_kv))
+        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: n_head %d / n_kv %d", in->n_head, n_kv);
+    if (!(in->freq_base > 1.0f) || std::isinf(in->freq_base))
         return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: freq_base must be finite and above 1");
-    if (B < 0 || n_tokens < 0 || (!seq_start && n_tokens != B))
-        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: B %d, n_tokens %d%s", B, n_tokens,
-                    seq_start ? "" : " without seq_start");
-    if ((int64_t)n_tokens * (n_head + 2 * (int64_t)cache->n_kv) >= (int64_t)1 << 31)
-        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: %d tokens of %d heads are too many", n_tokens, n_head);
-    if (B == 0 || n_tokens == 0) return VELO_OK;
-    if (!k || !v || !ctx_len || !q != !q_out || !q != (n_head == 0) || !k_out != !v_out)
+    if (in->B < 0 || in->n_tokens < 0 || (!in->seq_start && in->n_tokens != in->B))
+        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: B %d, n_tokens %d%s", in->B, in->n_tokens,
+                    in->seq_start ? "" : " without seq_start");
+    if ((int64_t)in->n_tokens * (in->n_head + 2 * (int64_t)n_kv) >= (int64_t)1 << 31)
+        return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: %d tokens of %d heads are too many", in->n_tokens, in->n_head);
+    if (in->B == 0 || in->n_tokens == 0) return VELO_OK;
+    if (!in->k || !in->v || !in->ctx_len || !in->q != !in->q_out || !in->q != (in->n_head == 0) || !in->k_out != !in->v_out)
         return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: NULL buffer");
-    const int eb = elem_bytes(in_dtype), D = cache->head_dim;
-    if ((q && (misaligned(q) || misaligned(q_out) || ldq * eb % 16)) || misaligned(k) || misaligned(v) ||
-        ldk * eb % 16 || ldv * eb % 16 || misaligned(k_out) || misaligned(v_out))
+    const int eb = elem_bytes(in->in_dtype);
+    if ((in->q && (misaligned(in->q) || misaligned(in->q_out) || in->ldq * eb % 16)) || misaligned(in->k) ||
+        misaligned(in->v) || in->ldk * eb % 16 || in->ldv * eb % 16 || misaligned(in->k_out) || misaligned(in->v_out) ||
+        misaligned(in->seq_start, 4) || misaligned(in->ctx_len, 4))
         return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: rows must be 16-byte aligned");
-    if ((q && ldq < (int64_t)n_head * D) || ldk < (int64_t)cache->n_kv * D || ldv < (int64_t)cache->n_kv * D)
+    if ((in->q && in->ldq < (int64_t)in->n_head * D) || in->ldk < (int64_t)n_kv * D || in->ldv < (int64_t)n_kv * D)
         return fail(VELO_ERR_INVALID_ARGUMENT, "kv_append: row stride below the row (ldq %lld, ldk %lld, ldv %lld)",
-                    (long long)ldq, (long long)ldk, (long long)ldv);
+                    (long long)in->ldq, (long long)in->ldk, (long long)in->ldv);
     DeviceScope dev(c->device);
     VELO_CUDA_TRY(dev.st);
-    a.q = q;
-    a.k = k;
-    a.v = v;
-    a.in_dtype = in_dtype;
-    a.ldq = ldq;
-    a.ldk = ldk;
-    a.ldv = ldv;
-    a.seq_start = seq_start;
-    a.ctx_len = ctx_len;
-    a.B = B;
-    a.T = n_tokens;
-    a.Hq = n_head;
-    a.q_out = q_out;
-    a.k_out = k_out;
-    a.v_out = v_out;
+    a.q = in->q;
+    a.k = in->k;
+    a.v = in->v;
+    a.in_dtype = in->in_dtype;
+    a.ldq = in->ldq;
+    a.ldk = in->ldk;
+    a.ldv = in->ldv;
+    a.seq_start = in->seq_start;
+    a.ctx_len = in->ctx_len;
+    a.B = in->B;
+    a.T = in->n_tokens;
+    a.Hq = in->n_head;
+    a.q_out = in->q_out;
+    a.k_out = in->k_out;
+    a.v_out = in->v_out;
     a.err = c->err_flag;
-    a.turns = rope_turns(c, freq_base, D);
+    a.turns = rope_turns(c, in->freq_base, D);
     VELO_CUDA_TRY(velo::launch_kv_append(a, c->sm_count, c->stream));
     return VELO_OK;
 }

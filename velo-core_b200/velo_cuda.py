@@ -11,6 +11,7 @@ analogues) and whose message is velo_cuda_last_error().
 import ctypes
 import os
 import re
+import struct
 
 import numpy as np
 
@@ -102,8 +103,7 @@ _SIGS = {
     "velo_cuda_gemm_q4_0": (_I32, [_P, _P, _P, _I32, _I32, _I32, _P, _I32, _I32]),
     "velo_cuda_tree_attention": (_I32, [_P, _P, _P, _P, _P, _P, _I32, _P, _I32, _P, _P, _P, _P,
                                         _I32, _I32, _I32, _I32, _I32, _I32, _P, _I32]),
-    "velo_cuda_kv_append": (_I32, [_P, _P, _P, _P, _P, _I32, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, _P, _P,
-                                   _I32, _I32, _I32, ctypes.c_float, _P, _P, _P]),
+    "velo_cuda_kv_append": (_I32, [_P, _P, _P]),
     "velo_cuda_decode_attention_workspace": (_SZ, [_P, _I32, _I32, _I32]),
     "velo_cuda_decode_attention": (_I32, [_P, _P, _P, ctypes.c_int64, _P, _I32, _I32, ctypes.c_float, _P, _P, _P,
                                           _SZ]),
@@ -185,6 +185,11 @@ class KvCacheDesc(ctypes.Structure):
     _fields_ = [("struct_size", ctypes.c_uint32), ("kv_dtype", _I32), ("k_pool", _P), ("v_pool", _P),
                 ("k_scale", _P), ("v_scale", _P), ("page_table", _P), ("pool_pages", _I32), ("max_pages", _I32),
                 ("n_kv", _I32), ("head_dim", _I32)]
+
+
+# velo_kv_append_batch: struct_size, in_dtype, q, k, v, ldq, ldk, ldv, seq_start, ctx_len, B, n_tokens, n_head,
+# freq_base, q_out, k_out, v_out
+_APPEND = struct.Struct("@IiPPPqqqPPiiifPPP")
 
 
 class VerifyBatch(ctypes.Structure):
@@ -279,16 +284,21 @@ def _tensor(what, t, types, code, shape, device):
 
 
 def _rows(what, t, code, shape, device):
-    """(address, row stride) of a tensor whose rows t[i] are dense and may have any
-    distance."""
+    """(address, row stride) of a tensor whose rows t[i] ([n] or [heads][dim]) are
+    dense and may have any distance."""
     st = t.stride()
-    if (_ELEMS[t.dtype] != code or t.shape != shape or t.get_device() != device or st[-1] != 1 or
-            (len(st) == 3 and st[1] != shape[2] and shape[1] != 1)):
+    if len(st) == 3:
+        step, row, last = st
+        width = shape[1] * shape[2]
+        dense = last == 1 and (row == shape[2] or shape[1] == 1)
+    else:
+        step, last = st
+        width = shape[1]
+        dense = last == 1 or width == 1
+    if not dense or _ELEMS[t.dtype] != code or t.shape != shape or t.get_device() != device:
         _refuse(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device}, strides {st}: not the element type, shape "
                 f"{tuple(shape)}, device {device} or dense rows needed")
-    if shape[0] > 1:
-        return t.data_ptr(), st[0]
-    return t.data_ptr(), shape[1] * shape[2] if len(st) == 3 else shape[1]
+    return t.data_ptr(), step if shape[0] > 1 else width
 
 
 class KvCache:
@@ -335,6 +345,8 @@ class Context:
                                      ctypes.byref(h)))
         self._h = h
         self.device = device
+        self._append = ctypes.create_string_buffer(_APPEND.size)
+        self._append_ref = ctypes.byref(self._append)
         self._kv_append = lib().velo_cuda_kv_append
         self._decode_attention = lib().velo_cuda_decode_attention
         self._token_logprobs = lib().velo_cuda_token_logprobs
@@ -450,14 +462,15 @@ class Context:
         if cache.device != dev or cache.rows < B or e < 0:
             _refuse(f"cache on device {cache.device} with {cache.rows} page-table rows, {B} sequences on device {dev}, "
                     f"k {k.dtype}")
-        pq = pqo = pko = pvo = pss = None
-        ldq = Hq = 0
+        pq = pqo = pko = pvo = pss = ldq = Hq = 0
         kv = (T, n, hd)
         if q is not None:
             Hq = q.shape[1]
             heads = (T, Hq, hd)
             pq, ldq = _rows("q", q, e, heads, dev)
             pqo = _tensor("q_out", q_out, _ELEMS, act, heads, dev)
+        elif q_out is not None:
+            _refuse("q_out without q")
         pk, ldk = _rows("k", k, e, kv, dev)
         pv, ldv = _rows("v", v, e, kv, dev)
         if k_out is not None or v_out is not None:
@@ -465,8 +478,9 @@ class Context:
             pvo = _tensor("v_out", v_out, _ELEMS, act, kv, dev)
         if seq_start is not None:
             pss = _tensor("seq_start", seq_start, _INTS, 0, (B + 1,), dev)
-        check(self._kv_append(self._h, cache.ref, pq, pk, pv, e, ldq, ldk, ldv, pss,
-                              _tensor("ctx_len", ctx_len, _INTS, 0, (B,), dev), B, T, Hq, freq_base, pqo, pko, pvo))
+        _APPEND.pack_into(self._append, 0, _APPEND.size, e, pq, pk, pv, ldq, ldk, ldv, pss,
+                          _tensor("ctx_len", ctx_len, _INTS, 0, (B,), dev), B, T, Hq, freq_base, pqo, pko, pvo)
+        check(self._kv_append(self._h, cache.ref, self._append_ref))
 
     def decode_attention_workspace(self, n_head, n_kv, head_dim):
         """Bytes of decode_attention's workspace, for any batch and lengths."""
