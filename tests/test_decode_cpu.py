@@ -58,16 +58,18 @@ class _Share:
         return u // (self.q + 1) if u < head else self.r + (u - head) // self.q
 
 
-def _ranges(units, per_seq, main, tail, whole=16, least=4, share=12, tail_units=64, tail_states=24):
+def _ranges(units, per_seq, main, tail, least=4, share=12, tail_units=64, tail_states=24, join=24):
     """decode_attn.cu's cut of the unit list: per block its pieces (item, first,
     last + 1 unit of the item, units, slot of a partial piece), and the open item
     with its last block."""
     pre = np.concatenate(([0], np.cumsum(np.asarray(units) * per_seq)))
     total = int(pre[-1])
+    n = min(main, -(-total // least))
+    uncut = -(-int(np.count_nonzero(units)) * per_seq // n) * int(max(units)) - total // n <= join
     if tail and total // main >= tail_units and max(units) <= tail_states * (total // share // tail):
         big, small = _Share(total - total // share, main), _Share(total // share, tail)
     else:
-        big, small = _Share(total, min(main, -(-total // least))), _Share(0, 0)
+        big, small = _Share(total, n), _Share(0, 0)
     blocks = big.k + small.k
 
     def item(u):
@@ -81,7 +83,7 @@ def _ranges(units, per_seq, main, tail, whole=16, least=4, share=12, tail_units=
         if c == 0 or u >= total:
             return u
         _, start, n = item(u)
-        return start if n <= max(whole, (big.q if c <= big.k else small.q) // 4) else u
+        return start if uncut or n <= max(join, (big.q if c <= big.k else small.q) // 4) else u
 
     def block_of(u):
         return big.range_of(u) if u < big.n else big.k + small.range_of(u - big.n)

@@ -31,6 +31,7 @@
 //  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
 //   dimensions for the output.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "common/elem.cuh"
@@ -50,9 +51,7 @@ constexpr int kErrSeqLen = 0x6211, kErrPage = 0x6212;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kMinUnits = 4;  // units per block at least: one per warp
-// An item of at most this many units (256 tokens of f16 pages), or of a quarter of
-// a block's range, is never cut.
-constexpr int kWholeUnits = 16;
+// Items of at most kJoinUnits (below), or of a quarter of a block's range, are never cut.
 constexpr int kRing = 64;  // unit descriptions per warp
 
 // Resident blocks per SM: INT8 pages with at most 8 query heads per KV head need
@@ -73,6 +72,9 @@ struct Layout {
     static constexpr int kHalf = kTok * kRow;                   // K, then V
     static constexpr int kStage = 2 * kHalf + (KV == VELO_KV_INT8 ? 4 * kTok : 0);  // + scales
     static constexpr int kStages = (blocks_per_sm(KV, R) == 3 ? 2 : 3) * (128 / D);
+    // What the join costs, in units of a block's time: items are only cut where whole ones would
+    // make some block later by more
+    static constexpr int kJoinUnits = (KV == VELO_KV_F16 ? 24 : KV == VELO_KV_INT8 ? 10 : 12) * (128 / D);
     static constexpr int kRings = kWarps * kStages * kStage;
     static constexpr int kStats = kRings + kWarps * kRing * 16;
     static constexpr int kQ = kStats + 3 * kWarps * 16 * 4;     // f32: q, and each warp's weights
@@ -204,6 +206,7 @@ struct Share {
 };
 struct Cut {
     Share big, tail;  // the large ranges, then the short ones
+    bool uncut;       // no item is cut
     __device__ __forceinline__ int blocks() const { return big.k + tail.k; }
     __device__ __forceinline__ int total() const { return big.n + tail.n; }
     __device__ __forceinline__ int at(int c) const { return c <= big.k ? big.at(c) : big.n + tail.at(c - big.k); }
@@ -212,24 +215,29 @@ struct Cut {
     }
     // Items up to this length are not cut by the start of block c (never more in the tail, so
     // that moving a cut to an item's start keeps the cuts in order).
-    __device__ __forceinline__ int whole(int c) const { return max(kWholeUnits, (c <= big.k ? big.q : tail.q) / 4); }
+    __device__ __forceinline__ int whole(int c, int least) const {
+        return uncut ? INT_MAX : max(least, (c <= big.k ? big.q : tail.q) / 4);
+    }
 };
-__device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int longest) {
-    const int tail = plan.blocks - plan.main;
+// items: how many there are, longest: units of the longest.
+__device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int items, int longest, int join_units) {
+    const int tail = plan.blocks - plan.main, blocks = min(plan.main, (total + kMinUnits - 1) / kMinUnits);
+    // whole items make the fullest block this much longer than an equal share
+    const bool uncut = total > 0 && (long long)((items + blocks - 1) / blocks) * longest - total / blocks <= join_units;
     if (tail > 0 && total / plan.main >= kTailUnits && longest <= kTailStates * (total / kTailShare / tail)) {
         const int n = total / kTailShare;
-        return Cut{Share(total - n, plan.main), Share(n, tail)};
+        return Cut{Share(total - n, plan.main), Share(n, tail), uncut};
     }
-    return Cut{Share(total, min(plan.main, (total + kMinUnits - 1) / kMinUnits)), Share(0, 0)};
+    return Cut{Share(total, blocks), Share(0, 0), uncut};
 }
 
 // First unit of block c: moved to the start of the item it falls into when that is short.
 template <int kTok>
-__device__ __forceinline__ int cut_at(const int* pre, const int* lens, int B, const Cut& k, int c) {
+__device__ __forceinline__ int cut_at(const int* pre, const int* lens, int B, const Cut& k, int join_units, int c) {
     const int u = c < k.blocks() ? k.at(c) : k.total();
     if (c == 0 || u >= k.total()) return u;
     const Item x = item_of<kTok>(pre, lens, B, u);
-    return x.units <= k.whole(c) ? x.start : u;
+    return x.units <= k.whole(c, join_units) ? x.start : u;
 }
 
 // KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item (0: half a tile).
@@ -250,14 +258,14 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
     int* stat_buf = reinterpret_cast<int*>(stat_l + kWarps * 16);
     int* lens = reinterpret_cast<int*>(smem + L::kLens);
     int* pre = lens + a.B;
-    __shared__ int s_warp[kWarps], s_long[kWarps], s_cut[2];
+    __shared__ int s_warp[kWarps], s_long[kWarps], s_filled[kWarps], s_cut[2];
     int4* desc = static_cast<int4*>(a.ws);
     float* slots = reinterpret_cast<float*>(desc + plan.blocks);
 
     // lengths and units before each sequence
     {
         const int per = (a.B + kThreads - 1) / kThreads, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
-        int sum = 0, longest = 0;
+        int sum = 0, longest = 0, filled = 0;
         for (int b = lo; b < hi; ++b) {
             int n = a.seq_len[b];
             if (n < 0 || n > a.kv.max_pages * kPageTokens) {
@@ -268,6 +276,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
             pre[b] = sum;
             sum += (n + kTok - 1) / kTok * per_seq;
             longest = max(longest, (n + kTok - 1) / kTok);
+            filled += n > 0;
         }
         int x = sum;
 #pragma unroll
@@ -275,10 +284,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        if (plan.blocks > plan.main) longest = __reduce_max_sync(0xffffffffu, longest);
+        longest = __reduce_max_sync(0xffffffffu, longest);
+        filled = __reduce_add_sync(0xffffffffu, filled);
         if (lane == 31) {
             s_warp[warp] = x;
             s_long[warp] = longest;
+            s_filled[warp] = filled;
         }
         __syncthreads();
         int before = x - sum;
@@ -288,7 +299,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         __syncthreads();
     }
     const int total = pre[a.B];
-    const Cut list = cut_list(plan, total, max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3])));
+    const Cut list = cut_list(plan, total, (s_filled[0] + s_filled[1] + s_filled[2] + s_filled[3]) * per_seq,
+                              max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3])), L::kJoinUnits);
 
     // sequences without tokens
     for (int b = c; b < a.B; b += gridDim.x) {
@@ -301,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         if (tid == 0) desc[c] = make_int4(-1, 0, 0, 0);
         return;
     }
-    if (tid < 2) s_cut[tid] = cut_at<kTok>(pre, lens, a.B, list, c + tid);
+    if (tid < 2) s_cut[tid] = cut_at<kTok>(pre, lens, a.B, list, L::kJoinUnits, c + tid);
     __syncthreads();
     const int u0 = s_cut[0], u1 = s_cut[1];
 
@@ -870,39 +882,43 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
 }
 
 // Joins the partial states of the item that block x of the first kernel left
-// open: slot 1 of that block, slot 0 of the following ones.  One block per (open
-// item, query head); each of its warps takes every fourth state, eight at a time
-// (maxima, sums and outputs in one round of reads, the running maximum as in the
-// first kernel), and the four results are added in order.
-template <typename Act, int D>
-__global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnArgs a, const Plan plan, int rows) {
-    __shared__ float acc[kWarps][D], s_m[kWarps], s_l[kWarps];
+// open: slot 1 of that block, slot 0 of the following ones.  A block's warps are
+// shared out over the `rows` query heads of its blockIdx.y; each of a head's warps
+// takes every per-th state, eight at a time (maxima, sums and outputs in one round
+// of reads, the running maximum as in the first kernel), and their results are
+// added in order.
+template <typename Act, int D, int kJoinWarps, int rows>
+__global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(const DecodeAttnArgs a, const Plan plan,
+                                                                      int item_rows) {
+    __shared__ float acc[kJoinWarps][D], s_m[kJoinWarps], s_l[kJoinWarps];
     dependent_wait();  // the first kernel is complete and visible
-    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr int per = kJoinWarps / rows;
+    const int row = blockIdx.y * rows + warp / per, part = warp % per;
     const int4* desc = static_cast<const int4*>(a.ws);
     const int4 it = desc[c];
     if (it.x < 0) return;
     const int hk = it.y / plan.tiles, tile = it.y % plan.tiles;
-    if (tile * rows + row >= plan.group) return;
-    const int head = hk * plan.group + tile * rows + row;
-    const size_t step = slot_floats(rows, D);
+    const bool live = tile * item_rows + row < plan.group;
+    const int head = hk * plan.group + tile * item_rows + row;
+    const size_t step = slot_floats(item_rows, D);
     const float* first = reinterpret_cast<const float*>(desc + plan.blocks) + (size_t)(2 * c) * step;
-    const int n = it.z - c + 1;
+    const int n = live ? it.z - c + 1 : 0;
     constexpr int kE = D / 32, kBatch = 8;
     float m = -INFINITY, l = 0.0f, x[kE] = {};
-    for (int i0 = warp; i0 < n; i0 += kWarps * kBatch) {
+    for (int i0 = part; i0 < n; i0 += per * kBatch) {
         float2 ml[kBatch];
         float o[kBatch][kE];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            const int i = i0 + j * kWarps;
+            const int i = i0 + j * per;
             ml[j] = make_float2(-INFINITY, 0.0f);
 #pragma unroll
             for (int e = 0; e < kE; ++e) o[j][e] = 0.0f;
             if (i < n) {
                 const float* st = first + (i == 0 ? 1 : 2 * (size_t)i) * step;
                 ml[j] = *reinterpret_cast<const float2*>(st + 2 * row);
-                const float* p = st + 2 * rows + row * D + lane * kE;
+                const float* p = st + 2 * item_rows + row * D + lane * kE;
                 if constexpr (kE == 4) {
                     const float4 v = *reinterpret_cast<const float4*>(p);
                     o[j][0] = v.x, o[j][1] = v.y, o[j][2] = v.z, o[j][3] = v.w;
@@ -935,19 +951,22 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const DecodeAttnA
 #pragma unroll
     for (int e = 0; e < kE; ++e) acc[warp][lane * kE + e] = x[e];
     __syncthreads();
-    float M = -INFINITY, L = 0.0f, f[kWarps];
+    if (part != 0 || !live) return;
+    float M = -INFINITY, L = 0.0f, y[kE] = {};
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_m[w]);
+    for (int w = 0; w < per; ++w) M = fmaxf(M, s_m[warp + w]);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        f[w] = ex2_approx(s_m[w] - (M == -INFINITY ? 0.0f : M));
-        L = fmaf(s_l[w], f[w], L);
+    for (int w = 0; w < per; ++w) {
+        const float f = ex2_approx(s_m[warp + w] - (M == -INFINITY ? 0.0f : M));
+        L = fmaf(s_l[warp + w], f, L);
+#pragma unroll
+        for (int e = 0; e < kE; ++e) y[e] = fmaf(acc[warp + w][lane * kE + e], f, y[e]);
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    for (int d = tid; d < D; d += kThreads)
-        static_cast<Act*>(a.out)[((size_t)it.x * a.Hq + head) * D + d] =
-            (Act)((acc[0][d] * f[0] + acc[1][d] * f[1] + acc[2][d] * f[2] + acc[3][d] * f[3]) * inv);
-    if (tid == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
+    Act* out = static_cast<Act*>(a.out) + ((size_t)it.x * a.Hq + head) * D + lane * kE;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) out[e] = (Act)(y[e] * inv);
+    if (lane == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
 int main_blocks(int kv, int R, int sm_count) {
@@ -975,10 +994,14 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) 
         items * kTailStates < (long long)kTailShare * (p.blocks - p.main))
         p.blocks = p.main;
     e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(p.blocks), kThreads, smem, 1, s, a, p);
-    if (e != cudaSuccess || most <= kWholeUnits) return e;  // no item of this table is ever cut
+    if (e != cudaSuccess || most <= L::kJoinUnits) return e;  // no item of this table is ever cut
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
-    return launch_dependent(decode_join_kernel<Act, D>, dim3(p.blocks, std::min(rows_of(R), p.group)), kThreads, 0, 1, s, a,
-                            p, rows_of(R));
+    // Few items are cut into many states each: 4 warps per query head.  Otherwise most blocks have
+    // nothing to join and only have to leave soon: one of 8 warps for (8 of) an item's heads.
+    constexpr int rows = rows_of(R), each = rows < 8 ? rows : 8;
+    if (items <= 16)
+        return launch_dependent(decode_join_kernel<Act, D, 4, 1>, dim3(p.blocks, rows), 128, 0, 1, s, a, p, rows);
+    return launch_dependent(decode_join_kernel<Act, D, 8, each>, dim3(p.blocks, rows / each), 256, 0, 1, s, a, p, rows);
 }
 
 template <int KV, int R>
