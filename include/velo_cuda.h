@@ -372,6 +372,7 @@ VELO_API int32_t velo_cuda_decode_attention(velo_cuda_ctx *ctx, const velo_kv_ca
  * asynchronous on the context stream.
  *   logits    [M][V] of logits_dtype (velo_elem), row m at m * ldl elements
  *   tokens    [M] u32 (NULL: no logprob)
+ *   temperature  in [1e-30, 1e30]
  *   logprob   [M] f32 (with tokens), entropy [M] f32 (or NULL)
  *   top_tokens [M][n_top] u32, top_logprobs [M][n_top] f32: the n_top largest
  *             logits in descending order, the lower index first among equal

@@ -449,6 +449,41 @@ def test_append_flags_bad_places(dctx):
     assert not pool[1].any()
     pool = run([[0], [1]], [0, 0], [1, 2, 3])         # token 0 belongs to no sequence
     assert pool[0, 0, 0].any() and pool[1, 0, 0].any() and not pool[0, 0, 1:].any()
+    pool = run([[0]], [5], [-2 ** 31, 3])             # a start far below zero puts every token past the row
+    assert not pool.any()
+
+
+def test_append_many_sequences_and_tiny_rows(dctx):
+    """More sequences than a block has threads (the two-level search), empty ones
+    among them; INT8 rows of zeros and of subnormal values."""
+    import torch
+    rng = np.random.default_rng(14)
+    B = 3000
+    new = rng.integers(0, 3, B)
+    cached = rng.integers(0, 14, B).astype(np.int32)
+    T = int(new.sum())
+    start = np.concatenate(([0], np.cumsum(new))).astype(np.int32)
+    v = rng.normal(0, 1, (T, 1, 64)).astype(np.float32)
+    v[::7] = 0
+    v[3::7] *= np.float32(1e-41)
+    table = rng.permutation(B).reshape(B, 1).astype(np.int32)
+    seq = np.repeat(np.arange(B), new)
+    sl = cached[seq] + np.arange(T) - start[seq]
+    for kv in ("f32", "int8"):
+        dt = torch.float32 if kv == "f32" else torch.int8
+        sc = [torch.zeros(B, 1, 16, dtype=torch.float16, device="cuda") for _ in range(2)] if kv == "int8" else [None] * 2
+        cache = velo_cuda.KvCache(torch.zeros(B, 1, 16, 64, dtype=dt, device="cuda"),
+                                  torch.zeros(B, 1, 16, 64, dtype=dt, device="cuda"), _dev(table), *sc)
+        dctx.kv_append(cache, None, _dev(v), _dev(v), _dev(cached), None, 10000.0, seq_start=_dev(start))
+        dctx.sync()
+        got = cache.tensors[1].cpu().numpy()[table[seq, 0], 0, sl].astype(np.float64)
+        if kv == "f32":
+            assert np.array_equal(got, v[:, 0].astype(np.float64))
+        else:
+            s = sc[1].cpu().numpy()[table[seq, 0], 0, sl].astype(np.float64)
+            m = np.abs(v[:, 0]).max(-1).astype(np.float64)
+            assert np.isfinite(s).all() and (np.abs(s - m / 127) <= _half_step(m / 127, True)).all()
+            assert (np.abs(got * s[:, None] - v[:, 0]) <= m[:, None] / 127 * 1.001 + np.abs(v[:, 0]) * 2.0 ** -10 + 2.0 ** -18).all()
 
 
 def test_append_refusals(dctx):
@@ -580,6 +615,26 @@ def test_logprobs_hard_rows(dctx, src):
         _check_logprobs(one, t[i:i + 1].float().numpy(), tokens[i:i + 1], n, 1.0)
 
 
+def test_logprobs_entropy_of_peaked_rows(dctx):
+    """A token that is nearly certain, wherever it lies: ln Z and Y / Z are both
+    near 0 when measured from it, so the small entropy keeps its digits."""
+    import torch
+    rng = np.random.default_rng(25)
+    V = 50021
+    x = rng.normal(0, 1, (24, V)).astype(np.float32)
+    for i in range(24):
+        x[i, int(rng.integers(0, V))] = [12, 15, 20, 30][i % 4]
+    tokens = x.argmax(-1)
+    for rows in (slice(0, 24), slice(3, 4)):
+        got = _score(dctx, torch.from_numpy(x[rows]), tokens[rows], 3, 1.0)
+        lp, ent, _, _ = ref.logprobs(x[rows], tokens[rows], 3, 1.0)
+        # the peak's thread adds a sum per 16 elements and its neighbours' to 1: (V / 4096 + 32)
+        # roundings of 2^-25; the other terms keep 2^-17 of themselves
+        tol = (V / 4096 + 32) * 2.0 ** -25
+        assert (np.abs(got[0] - lp) <= np.abs(lp) * 2.0 ** -17 + tol).all()
+        assert (np.abs(got[1] - ent) <= ent * 2.0 ** -17 + 2 * tol).all()
+
+
 @pytest.mark.parametrize("src", ["f32", "bf16"])
 @pytest.mark.parametrize("pad,shift", [(3, 0), (8, 0), (5, 1), (16, 4)])
 def test_logprobs_strides_and_alignment(dctx, src, pad, shift):
@@ -645,6 +700,76 @@ def test_logprobs_sampling_temperature_is_the_accept_distribution(dctx):
     want = torch.log_softmax(t.double() / 0.8, -1).gather(1, ids.long())
     assert (tl.double() - want).abs().max() < 1e-5
     assert torch.equal(ids.long().sort(-1).values, torch.arange(50, device="cuda").expand(4, 50))
+
+
+# ------------------------------------------------------------------ order on streams
+
+def test_calls_wait_for_what_precedes_them(dctx):
+    """The operators start as dependents of the kernel before them: they still see
+    copies, clears, other streams' work and each other's results."""
+    import torch
+    rng = np.random.default_rng(41)
+    B, H, D, V = 4, 2, 64, 70000
+    table = torch.arange(B * 4, dtype=torch.int32, device="cuda").view(B, 4)
+    cache = velo_cuda.KvCache(torch.zeros(B * 4, H, 16, D, device="cuda"), torch.zeros(B * 4, H, 16, D, device="cuda"), table)
+    src = [_dev(rng.normal(0, 1, (B, 3 * H, D)).astype(np.float32)) for _ in range(3)]
+    x, q = torch.empty_like(src[0]), torch.empty(B, H, D, device="cuda")
+    out, ws = torch.empty_like(q), torch.empty(dctx.decode_attention_workspace(H, H, D), dtype=torch.uint8, device="cuda")
+    pos, lens = (torch.zeros(B, dtype=torch.int32, device="cuda") for _ in range(2))
+    logits, lp = torch.zeros(B, V, device="cuda"), torch.empty(B, device="cuda")
+    tok = torch.zeros(B, dtype=torch.int32, device="cuda")
+    big = torch.zeros(1 << 26, device="cuda")
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+
+    def step(i, n):
+        with torch.cuda.stream(side):
+            side.wait_stream(main)
+            big.add_(1.0)                       # a slow kernel before the rows are ready
+            x.copy_(src[i])
+        main.wait_stream(side)
+        dctx.kv_append(cache, x[:, :H], x[:, H:2 * H], x[:, 2 * H:], pos, q, 10000.0)
+        pos.add_(1)
+        lens.copy_(pos)
+        dctx.decode_attention(cache, q, lens, out, ws)
+        logits.zero_()
+        logits[:, :H * D].copy_(out.view(B, -1))
+        dctx.token_logprobs(logits, tok, lp)
+        return lp.clone(), out.clone()
+    results = []
+    for rounds in range(3):
+        with torch.cuda.stream(main):
+            dctx.set_stream(main.cuda_stream)
+            pos.zero_()
+            got = [step(i % 3, i) for i in range(20)]
+        torch.cuda.synchronize()
+        results.append(torch.cat([t.flatten() for r in got for t in r]).cpu())
+    dctx.sync()
+    assert all(torch.equal(r, results[0]) for r in results)
+    last = results[0][-B * H * D:].view(B, H, D).numpy()
+    # the last step against 64 bits, over the twenty cached rows
+    k, v = cache.tensors[0].cpu().numpy(), cache.tensors[1].cpu().numpy()
+    want, _, _, vmax = ref.attention(q.cpu().numpy(), k, v, table.cpu().numpy(), [20] * B)
+    assert np.abs(last - want).max() <= 1e-5 * vmax
+    rows = np.stack([src[i % 3].cpu().numpy()[:, 2 * H:] for i in range(20)], 1)  # [B][20][H][D]
+    assert np.array_equal(np.moveaxis(v[table.cpu().numpy()], 3, 2).reshape(B, -1, H, D)[:, :20], rows)
+    # the same chain captured: a clear, a copy and the operators as graph nodes
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        pos.zero_()
+        x.zero_()
+        x.copy_(src[1])
+        dctx.kv_append(cache, x[:, :H], x[:, H:2 * H], x[:, 2 * H:], pos, q, 10000.0)
+        lens.copy_(pos).add_(1)
+        dctx.decode_attention(cache, q, lens, out, ws)
+    dctx.set_stream(velo_cuda.DEFAULT_STREAM)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        # one cached token: the output is its V row
+        assert torch.equal(out, src[1][:, 2 * H:])
 
 
 # ------------------------------------------------------------------ together

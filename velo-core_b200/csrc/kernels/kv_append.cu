@@ -92,9 +92,9 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
         if (threadIdx.x == 0) atomicCAS(a.err, 0, kErrAppend);
         return;
     }
-    const long long pos = (long long)cached + (t - first);
+    const long long pos = (long long)cached + ((long long)t - first);
     const int pi = (int)(pos / kPageTokens), slot = (int)(pos % kPageTokens);
-    bool ok = cached >= 0 && pos / kPageTokens < a.kv.max_pages;
+    bool ok = cached >= 0 && pos >= 0 && pos / kPageTokens < a.kv.max_pages;
     uint32_t page = 0;
     if (ok) page = a.kv.page_table[(size_t)b * a.kv.max_pages + pi];
     if (threadIdx.x < D / 2) {
@@ -141,7 +141,8 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
 #pragma unroll
             for (int o = kLanes / 2; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             if (!live || is_q) continue;
-            const float inv = mx > 0.0f ? __fdiv_rn(127.0f, mx) : 0.0f;
+            float inv = mx > 0.0f ? __fdiv_rn(127.0f, mx) : 0.0f;
+            if (inv == INFINITY) inv = 0.0f;  // a row below 2^-121: its scale is 0 as well
             const __half scale = __float2half_rn(__fdiv_rn(mx, 127.0f));
             uint32_t w0[2] = {0, 0}, w1[2] = {0, 0};
 #pragma unroll

@@ -1,7 +1,7 @@
 // token_logprobs.cu -- log probability of given tokens, entropy and the best
 // alternatives of each logits row (velo_cuda_token_logprobs).
 //
-// With m close to the row's maximum, k = log2(e) / T, u = (x - m) k: Z = sum 2^u, Y = sum u 2^u,
+// With m the row's maximum so far, k = log2(e) / T, u = (x - m) k: Z = sum 2^u, Y = sum u 2^u,
 // log probability = (x[token] - m) / T - ln Z, entropy = ln Z - ln 2 Y / Z.
 // Each logit is read once from HBM, which bounds the kernel.
 //
@@ -114,7 +114,7 @@ __device__ __forceinline__ void unpack(const __nv_bfloat16*, uint4 v, float* x) 
     }
 }
 
-// Running sums: m is a logit near the largest, Z and Y belong to u = (x - m) k.  (x - m
+// Running sums: m is the largest logit, Z and Y belong to u = (x - m) k.  (x - m
 // rather than one fma: a row masked with the type's lowest value must not overflow.)
 struct Sums {
     float m, z, y;
@@ -264,9 +264,7 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
         s.z += z.x;
         s.y += y.x;
     }
-    // m is raised only when 2^u could pass 2^8, so that few tiles rescale the sums
-    const float slack = 8.0f / k;
-    float best = s.m, piece = -INFINITY, limit = s.m + slack;
+    float best = s.m, piece = -INFINITY;
     int left = per_slot, slot = tid;  // tiles left of the piece, its place in slot_max
     uint32_t stage = 0;
     auto consume = [&](int tile, auto whole) {
@@ -296,10 +294,12 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
         }
         m = max3(max3(m, m1, piece), x[kVecs * kN - 2], x[kVecs * kN - 1]);
         piece = m;
-        if (__any_sync(0xffffffffu, m > limit)) {
-            raise(s, m, k);
-            limit = s.m + slack;
-        }
+        // the sums at the new maximum (a reference below it would cost the entropy of a peaked row its
+        // digits: ln Z and Y / Z would both be large); -inf - -inf and -inf * 0 become factors of 0
+        const float top = fmaxf(s.m, m), d = fmaxf((s.m - top) * k, -200.0f), f = ex2_approx(d);
+        s.m = top;
+        s.y = f * fmaf(d, s.z, s.y);
+        s.z *= f;
         const float2 minus_m = f2(-base_of(s.m));
         float2 z = f2(0.0f), y = f2(0.0f);
 #pragma unroll

@@ -42,7 +42,7 @@ int32_t check_cache(const char* op, const velo_kv_cache* k, velo::PagedKv& out) 
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: kv_dtype %d", op, k->kv_dtype);
     if (k->head_dim != 64 && k->head_dim != 128)
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: head_dim %d unsupported (64 or 128)", op, k->head_dim);
-    if (k->n_kv < 1 || k->pool_pages < 1 || k->max_pages < 0)
+    if (k->n_kv < 1 || k->pool_pages < 1 || k->max_pages < 0 || k->max_pages > 1 << 26)
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: n_kv %d, pool_pages %d, max_pages %d", op, k->n_kv,
                     k->pool_pages, k->max_pages);
     if (!k->k_pool || !k->v_pool || (k->max_pages > 0 && !k->page_table) ||
@@ -202,8 +202,8 @@ int32_t velo_cuda_token_logprobs(velo_cuda_ctx* c, const void* logits, int32_t l
     if (n_top < 0 || n_top > velo::kMaxTop || n_top > V)
         return fail(VELO_ERR_INVALID_ARGUMENT, "token_logprobs: n_top = %d outside [0, min(%d, V)]", n_top,
                     velo::kMaxTop);
-    if (!(temperature > 0.0f) || std::isinf(temperature) || std::isinf(1.0f / temperature))
-        return fail(VELO_ERR_INVALID_ARGUMENT, "token_logprobs: temperature must be finite and > 0");
+    if (!(temperature >= 1e-30f && temperature <= 1e30f))
+        return fail(VELO_ERR_INVALID_ARGUMENT, "token_logprobs: temperature outside [1e-30, 1e30]");
     if (ldl < V) return fail(VELO_ERR_INVALID_ARGUMENT, "token_logprobs: ldl %lld < V = %d", (long long)ldl, V);
     if (M == 0) return VELO_OK;
     if (!logits || !tokens != !logprob || (n_top > 0 && (!top_tokens || !top_logprobs)))
