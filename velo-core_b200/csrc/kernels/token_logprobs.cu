@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
     constexpr int kN = Vec<T>::n, kWarps = S::kWarps, kTileVecs = S::kTileVecs;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums s_part[kWarps];
-    __shared__ uint32_t s_bound[kWarps * 32];
+    __shared__ __align__(16) uint32_t s_bound[kWarps * 32 + 4];
     __shared__ int s_count, s_work, s_warp[kWarps];
     __shared__ unsigned long long s_raise;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -363,6 +363,7 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
         const int full_warps = min(kWarps, nv / 32);  // warps whose every lane has data
         const int keep = full_warps ? min(32, (a.n_top + full_warps - 1) / full_warps + 2) : 0;
         const int kept = full_warps * keep;
+        if (tid < 4) s_bound[kept + tid] = 0;  // read with the last ones, below all
         uint32_t key = order_key(best);
         for (int i = 0; i < keep; ++i) {
             const uint32_t top = __reduce_max_sync(0xffffffffu, key);
@@ -377,7 +378,12 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
             for (int i = lane; i < (kept + 31) / 32 * 32; i += 32) {
                 const uint32_t v = i < kept ? s_bound[i] : 0u;
                 int rank = 0;
-                for (int j = 0; j < kept; ++j) rank += s_bound[j] > v || (s_bound[j] == v && j < i);
+#pragma unroll 2
+                for (int j = 0; j < kept; j += 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(s_bound + j);
+                    rank += (x.x > v) + (x.y > v) + (x.z > v) + (x.w > v);
+                    rank += (x.x == v && j < i) + (x.y == v && j + 1 < i) + (x.z == v && j + 2 < i) + (x.w == v && j + 3 < i);
+                }
                 const uint32_t hit = __ballot_sync(0xffffffffu, i < kept && rank == a.n_top - 1);
                 if (hit) {
                     bound = __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
@@ -434,6 +440,7 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
         post_sums();
         __syncthreads();
     }
+    if (cluster == 1 && warp > 0 && warp * 32 >= c) return;  // nothing to write
     s = warp_join(s_part[lane % kWarps], k, kWarps);
     s.m = __shfl_sync(0xffffffffu, s.m, 0);
     s.z = __shfl_sync(0xffffffffu, s.z, 0);
