@@ -161,6 +161,15 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
 __device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
 __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return even_bytes(w >> 8); }
 
+// a / b, a >= 0 and b > 0: below 2^22 the f32 quotient is within one of it, which the
+// remainder settles (a third of an integer division's latency; a block starts with a
+// chain of these).
+__device__ __forceinline__ int quotient(int a, int b) {
+    if (a >= 1 << 22) return a / b;
+    const int q = (int)__fdividef((float)a, (float)b), r = a - q * b;
+    return q + (r >= b) - (r < 0);
+}
+
 // The largest b with pre[b] <= u.
 __device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
     int lo = 0, hi = B;
@@ -182,7 +191,7 @@ __device__ __forceinline__ Item item_of(const int* pre, const int* lens, int B, 
     Item x;
     x.b = find_sequence(pre, B, u);
     x.units = (lens[x.b] + kTok - 1) / kTok;
-    x.it = (u - pre[x.b]) / x.units;
+    x.it = quotient(u - pre[x.b], x.units);
     x.start = pre[x.b] + x.it * x.units;
     return x;
 }
@@ -198,10 +207,10 @@ constexpr int kTailStates = 24;                  // most short ranges of an item
 // n units in k ranges: the first n % k have one unit more.
 struct Share {
     int n, k, q, r;
-    __device__ __forceinline__ Share(int n_, int k_) : n(n_), k(k_), q(k_ ? n_ / k_ : 0), r(n_ - q * k_) {}
+    __device__ __forceinline__ Share(int n_, int k_) : n(n_), k(k_), q(k_ ? quotient(n_, k_) : 0), r(n_ - q * k_) {}
     __device__ __forceinline__ int at(int c) const { return c * q + min(c, r); }  // first unit of range c
     __device__ __forceinline__ int range_of(int u) const {
-        return u < r * (q + 1) ? u / (q + 1) : r + (u - r * (q + 1)) / q;
+        return u < r * (q + 1) ? quotient(u, q + 1) : r + quotient(u - r * (q + 1), q);
     }
 };
 struct Cut {
@@ -222,13 +231,16 @@ struct Cut {
 // items: how many there are, longest: units of the longest.
 __device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int items, int longest, int join_units) {
     const int tail = plan.blocks - plan.main, blocks = min(plan.main, (total + kMinUnits - 1) / kMinUnits);
+    const Share even(total, blocks);
     // whole items make the fullest block this much longer than an equal share
-    const bool uncut = total > 0 && (long long)((items + blocks - 1) / blocks) * longest - total / blocks <= join_units;
-    if (tail > 0 && total / plan.main >= kTailUnits && longest <= kTailStates * (total / kTailShare / tail)) {
+    const bool uncut =
+        total > 0 && (long long)quotient(items + blocks - 1, blocks) * longest - even.q <= join_units;
+    if (tail > 0 && quotient(total, plan.main) >= kTailUnits &&
+        longest <= kTailStates * quotient(total / kTailShare, tail)) {
         const int n = total / kTailShare;
         return Cut{Share(total - n, plan.main), Share(n, tail), uncut};
     }
-    return Cut{Share(total, blocks), Share(0, 0), uncut};
+    return Cut{even, Share(0, 0), uncut};
 }
 
 // First unit of block c: moved to the start of the item it falls into when that is short.
@@ -258,32 +270,53 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
     int* stat_buf = reinterpret_cast<int*>(stat_l + kWarps * 16);
     int* lens = reinterpret_cast<int*>(smem + L::kLens);
     int* pre = lens + a.B;
-    __shared__ int s_warp[kWarps], s_long[kWarps], s_filled[kWarps], s_cut[2];
+    __shared__ int s_warp[kWarps], s_long[kWarps], s_filled[kWarps];
     int4* desc = static_cast<int4*>(a.ws);
     float* slots = reinterpret_cast<float*>(desc + plan.blocks);
 
     // lengths and units before each sequence
-    {
-        const int per = (a.B + kThreads - 1) / kThreads, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
-        int sum = 0, longest = 0, filled = 0;
-        for (int b = lo; b < hi; ++b) {
-            int n = a.seq_len[b];
-            if (n < 0 || n > a.kv.max_pages * kPageTokens) {
-                if (c == 0) atomicCAS(a.err, 0, kErrSeqLen);
-                n = n < 0 ? 0 : a.kv.max_pages * kPageTokens;
-            }
-            lens[b] = n;
-            pre[b] = sum;
-            sum += (n + kTok - 1) / kTok * per_seq;
-            longest = max(longest, (n + kTok - 1) / kTok);
-            filled += n > 0;
+    auto length_of = [&](int b) {
+        int n = a.seq_len[b];
+        if (n < 0 || n > a.kv.max_pages * kPageTokens) {
+            if (c == 0) atomicCAS(a.err, 0, kErrSeqLen);
+            n = n < 0 ? 0 : a.kv.max_pages * kPageTokens;
         }
-        int x = sum;
+        return n;
+    };
+    auto running_sum = [&](int x) {
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
+        return x;
+    };
+    int total, longest, filled;
+    if (a.B <= 32) {  // every warp by itself, all with the same results: no barrier
+        const int n = lane < a.B ? length_of(lane) : 0, units = (n + kTok - 1) / kTok;
+        const int x = running_sum(units * per_seq);
+        if (lane < a.B) {
+            lens[lane] = n;
+            pre[lane] = x - units * per_seq;
+        }
+        total = __shfl_sync(0xffffffffu, x, 31);
+        if (lane == 0) pre[a.B] = total;
+        longest = __reduce_max_sync(0xffffffffu, units);
+        filled = __popc(__ballot_sync(0xffffffffu, n > 0));
+        __syncwarp();
+    } else {
+        const int per = (a.B + kThreads - 1) / kThreads, lo = min(tid * per, a.B), hi = min(lo + per, a.B);
+        int sum = 0;
+        longest = filled = 0;
+        for (int b = lo; b < hi; ++b) {
+            const int n = length_of(b), units = (n + kTok - 1) / kTok;
+            lens[b] = n;
+            pre[b] = sum;
+            sum += units * per_seq;
+            longest = max(longest, units);
+            filled += n > 0;
+        }
+        const int x = running_sum(sum);
         longest = __reduce_max_sync(0xffffffffu, longest);
         filled = __reduce_add_sync(0xffffffffu, filled);
         if (lane == 31) {
@@ -293,14 +326,19 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         }
         __syncthreads();
         int before = x - sum;
-        for (int w = 0; w < warp; ++w) before += s_warp[w];
+        longest = filled = 0;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) before += s_warp[w];
+            longest = max(longest, s_long[w]);
+            filled += s_filled[w];
+        }
         for (int b = lo; b < hi; ++b) pre[b] += before;
         if (tid == kThreads - 1) pre[a.B] = before + sum;
         __syncthreads();
+        total = pre[a.B];
     }
-    const int total = pre[a.B];
-    const Cut list = cut_list(plan, total, (s_filled[0] + s_filled[1] + s_filled[2] + s_filled[3]) * per_seq,
-                              max(max(s_long[0], s_long[1]), max(s_long[2], s_long[3])), L::kJoinUnits);
+    const Cut list = cut_list(plan, total, filled * per_seq, longest, L::kJoinUnits);
 
     // sequences without tokens
     for (int b = c; b < a.B; b += gridDim.x) {
@@ -313,9 +351,8 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         if (tid == 0) desc[c] = make_int4(-1, 0, 0, 0);
         return;
     }
-    if (tid < 2) s_cut[tid] = cut_at<kTok>(pre, lens, a.B, list, L::kJoinUnits, c + tid);
-    __syncthreads();
-    const int u0 = s_cut[0], u1 = s_cut[1];
+    const int edge = lane < 2 ? cut_at<kTok>(pre, lens, a.B, list, L::kJoinUnits, c + lane) : 0;
+    const int u0 = __shfl_sync(0xffffffffu, edge, 0), u1 = __shfl_sync(0xffffffffu, edge, 1);
 
     // ---- this warp's stream of units
     const int n_w = max(0, (u1 - u0 - warp + kWarps - 1) / kWarps);
