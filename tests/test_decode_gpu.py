@@ -153,6 +153,46 @@ def test_attention_long_split(dctx, kv):
     _check_attention(out, lse, q, d, lens, kv)
 
 
+@pytest.mark.parametrize("kv,B,Hq", [("f16", 40, 32), ("int8", 96, 16)])
+def test_attention_long_list_with_its_tail(dctx, kv, B, Hq):
+    """Enough work for the short ranges at the list's end: items cut in both parts."""
+    rng = np.random.default_rng(10)
+    lens = [int(n) for n in rng.integers(1000, 1500, B)]
+    d = _cache(rng, kv, lens, 8, 64)
+    q = rng.normal(0, 1.5, (B, Hq, 64)).astype(np.float16)
+    out, lse = _attend(dctx, d, q, lens)
+    _check_attention(out, lse, q, d, lens, kv)
+    again, lse2 = _attend(dctx, d, q, lens)
+    assert np.array_equal(out, again) and np.array_equal(lse, lse2)
+
+
+def test_attention_shared_prefix_pages(dctx):
+    """Sequences whose tables name the same pages, and a page named twice."""
+    rng = np.random.default_rng(15)
+    d = _cache(rng, "f16", [70, 70, 70], 2, 128, poison=False)
+    d["table"][1, :4] = d["table"][0, :4]
+    d["table"][2, :5] = d["table"][0, [0, 1, 1, 0, 4]]
+    q = rng.normal(0, 1, (3, 4, 128)).astype(np.float16)
+    out, lse = _attend(dctx, d, q, [70, 64, 66])
+    _check_attention(out, lse, q, d, [70, 64, 66], "f16")
+
+
+def test_attention_int8_scales_of_any_size(dctx):
+    """V scales from subnormal to large within one context, negative and zero ones."""
+    rng = np.random.default_rng(16)
+    lens = [333, 90, 40]
+    d = _cache(rng, "int8", lens, 2, 128, poison=False)
+    for b, n in enumerate(lens):
+        for t in range(n):
+            f = [[1e-3, 1.0, 300.0][t % 3], 2.0 ** -20, 0.0][b] * (-1 if t % 5 == 0 else 1)
+            d["v_scale"][d["table"][b, t // 16], :, t % 16] *= np.float16(f)
+    q = rng.normal(0, 1, (3, 8, 128)).astype(np.float16)
+    out, lse = _attend(dctx, d, q, lens)
+    _check_attention(out[:1], lse[:1], q[:1], dict(d, table=d["table"][:1]), lens[:1], "int8")
+    _check_attention(out[1:2], lse[1:2], q[1:2], dict(d, table=d["table"][1:2]), lens[1:2], "int8")
+    assert (out[2] == 0).all() and np.isfinite(lse[2]).all()
+
+
 def test_attention_many_sequences(dctx):
     rng = np.random.default_rng(4)
     lens = [int(x) for x in rng.integers(0, 40, 4096)]
@@ -292,6 +332,25 @@ def test_attention_other_stream_and_graph(dctx):
     torch.cuda.synchronize()
     _check_attention(runs[0][1].cpu().numpy(), runs[0][2].cpu().numpy(), q, d, [17, 0], "f16")
     dctx.set_stream(velo_cuda.DEFAULT_STREAM)
+
+
+def test_structs_of_another_size_are_refused(dctx):
+    import ctypes
+
+    import torch
+    z = torch.zeros(1, 1, 16, 64, device="cuda")
+    cache = velo_cuda.KvCache(z, z.clone(), torch.zeros(1, 1, dtype=torch.int32, device="cuda"))
+    L, bad = velo_cuda.lib(), velo_cuda.ERR_INVALID_ARGUMENT
+    batch = ctypes.create_string_buffer(velo_cuda._APPEND.size)
+    assert L.velo_cuda_kv_append(dctx.handle, cache.ref, ctypes.byref(batch)) == bad and "struct_size" in velo_cuda.last_error()
+    assert L.velo_cuda_kv_append(dctx.handle, cache.ref, None) == bad
+    assert L.velo_cuda_kv_append(dctx.handle, None, ctypes.byref(batch)) == bad
+    for field, value in (("struct_size", 8), ("kv_dtype", 3), ("head_dim", 96), ("n_kv", 0), ("pool_pages", 0), ("max_pages", -1),
+                         ("max_pages", (1 << 26) + 1), ("k_pool", None), ("page_table", None)):
+        d = velo_cuda.KvCacheDesc.from_buffer_copy(cache.desc)
+        setattr(d, field, value)
+        assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(d), None, 0, None, 1, 1, 0.0, None, None, None, 0) == bad
+    assert L.velo_cuda_decode_attention(dctx.handle, cache.ref, None, 64, None, 5000, 1, 0.0, None, None, None, 0) == bad
 
 
 # ------------------------------------------------------------------ append
@@ -540,7 +599,7 @@ def _score(ctx, t, tokens, n, T, dev=None):
 def _check_logprobs(got, x, tokens, n, T):
     lp, ent, ids, tlp = ref.logprobs(x, tokens, n, T)
     V = x.shape[1]
-    fin = np.where(np.isfinite(x), np.abs(x), 0).max(-1) / T
+    fin = np.where(np.isfinite(x), np.abs(x), 0).max(-1).astype(np.float64) / T
     # sums of exponentials: chains of V / 256 + 64 additions; an argument x / T - m: three
     # roundings of its size; the exponential itself 2^-21
     chain = (V / 256 + 64) * EPS + 2.0 ** -20
@@ -551,7 +610,7 @@ def _check_logprobs(got, x, tokens, n, T):
         ok = np.isfinite(b)
         assert np.array_equal(np.isnan(a), np.isnan(b)) and (a[~ok & ~np.isnan(b)] == b[~ok & ~np.isnan(b)]).all()
         t = np.broadcast_to(t, b.shape)
-        err = np.abs(a - b)[ok]
+        err = np.abs(a[ok] - b[ok])
         assert (err <= t[ok]).all(), (err / t[ok]).max()
     near(got[0], lp, tol)
     near(got[1], ent, tol * spread)
@@ -563,7 +622,8 @@ def _check_logprobs(got, x, tokens, n, T):
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("M,V,n,T", [(1, 1, 1, 1.0), (3, 5, 5, 0.5), (2, 64, 64, 1.0), (7, 1000, 20, 0.8), (1, 128256, 5, 1.0),
                                      (33, 32000, 8, 1.0), (5, 50257, 20, 0.7), (300, 4096, 3, 1.0), (2, 131071, 33, 1.3),
-                                     (700, 2049, 0, 1.0)])
+                                     (700, 2049, 0, 1.0), (2, 1 << 20, 20, 1.0), (5000, 33, 20, 1.0),
+                                     (700, 4093, 33, 0.9)])
 def test_logprobs_match_plain(dctx, src, M, V, n, T):
     rng = np.random.default_rng(M * 7 + V)
     t = _logits(rng, M, V, src)
@@ -574,30 +634,32 @@ def test_logprobs_match_plain(dctx, src, M, V, n, T):
     assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(got, again))
 
 
+@pytest.mark.parametrize("V,copies", [(20011, 1), (4001, 40)])
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
-def test_logprobs_hard_rows(dctx, src):
-    """Masked, tied, ordered and non-finite rows, each among ordinary ones."""
+def test_logprobs_hard_rows(dctx, src, V, copies):
+    """Masked, tied, ordered and non-finite rows, each among ordinary ones; many
+    copies of them take the smaller blocks."""
     import torch
-    V, n = 20011, 20
+    n = 20
     rng = np.random.default_rng(21)
     x = rng.normal(0, 2, (17, V)).astype(np.float32)
     x[0] = -np.inf                                  # nothing left
     x[1, :] = -np.inf
-    x[1, 7000] = 3                                  # one survivor
+    x[1, V // 3] = 3                                # one survivor
     x[2, 5:] = -np.inf                              # fewer than n survivors
     x[3] = 0                                        # all equal: the lowest indices
     x[4] = np.arange(V) * 1e-3                      # rising: every element beats all before
     x[5] = -np.arange(V) * 1e-3
     x[6] = np.rint(x[6])                            # many ties
     x[7, 100] = np.nan
-    x[8, 19999] = np.inf
+    x[8, V - 12] = np.inf
     x[9] = np.nan
     x[10, ::2] = -0.0
     x[10, 1::2] = 0.0                               # -0 and 0 are equal
     x[11] = -60000                                  # the lowest values as a mask
     x[11, 11::1000] = 1
     x[12] = 0
-    x[12, 9000:9064] = 5                            # the best lie side by side (one thread's loads)
+    x[12, V // 2:V // 2 + 64] = 5                   # the best lie side by side (one thread's loads)
     x[13] = 0
     x[13, 3::256] = 9                               # ... and one to a stride
     x[14, :] = np.where(np.arange(V) % 1024 < 4, 8 + x[14], x[14] - 8)
@@ -607,10 +669,11 @@ def test_logprobs_hard_rows(dctx, src):
         x[16, 5] = -2.9e38
     t = torch.from_numpy(x).to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[src])
     tokens = np.arange(17) * 1000 % V
-    tokens[1] = 7000
-    got = _score(dctx, t, tokens, n, 1.0)
-    _check_logprobs(got, t.float().numpy(), tokens, n, 1.0)
-    for i in range(17):  # one row alone takes the other split of the work
+    tokens[1] = V // 3
+    got = _score(dctx, t.repeat(copies, 1), np.tile(tokens, copies), n, 1.0)
+    for c in range(copies):  # (an odd V: the copies start at different offsets, so sums may group differently)
+        _check_logprobs([g[c * 17:(c + 1) * 17] for g in got], t.float().numpy(), tokens, n, 1.0)
+    for i in range(17 if copies == 1 else 0):  # one row alone takes the other split of the work
         one = _score(dctx, t[i:i + 1], tokens[i:i + 1], n, 1.0)
         _check_logprobs(one, t[i:i + 1].float().numpy(), tokens[i:i + 1], n, 1.0)
 

@@ -30,6 +30,12 @@
 //   split into two bf16 parts, whose exponent holds any scale.
 //  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
 //   dimensions for the output.
+//
+// Measured on a B200 against 6552 GB/s: 64 sequences of 3900 - 4290 f16 tokens, 64/8
+// heads, 168 us back to back (0.98); one of 100003 tokens 73 us (0.86: start-up and
+// join); 128 ragged INT8 sequences, 32/8 heads, 207 us at full clock (0.86), 220 - 235
+// at the 1500 MHz that the power cap leaves; one of 203 tokens 6.5 us, which is
+// latency: length, page and K/V reads in a row, four steps of a warp, the launch.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -492,8 +498,9 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                 }
             }
         }
-        // INT8: the scores carry 128 times the sum of q, which comes off each of them (against |q.k|
-        // it is small enough: 128 |sum q| is a few times 127 |q|)
+        // INT8: the scores carry 128 times the sum of q, which comes off each of them.  Their f32 sums
+        // are then as exact as those of a K row whose values all have its maximum's size: 2^-24 of
+        // sum |q| max|k| a step, far below the page's own rounding (max|k| / 127).
         float q128[kH][2];
         if constexpr (KV == VELO_KV_INT8) {
 #pragma unroll

@@ -13,6 +13,10 @@
 // finding its place (sequence, page, angles) and its rows, so six blocks per SM
 // matter more than loads moved up within one (measured: 13.5 us against 11.6 for
 // 2048 tokens of INT8 pages).
+//
+// Measured on a B200 against 6552 GB/s: 8533 prompt tokens of 32/32 heads, f32 to f16
+// pages, 95 us (1.0); 2048 tokens of 32/8 heads, bf16 to INT8, 12.2 us (0.68, latency);
+// 64 single tokens of 64/8 heads 3.2 us.
 #include <algorithm>
 
 #include "common/elem.cuh"

