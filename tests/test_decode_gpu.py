@@ -623,7 +623,8 @@ def _check_logprobs(got, x, tokens, n, T):
 @pytest.mark.parametrize("M,V,n,T", [(1, 1, 1, 1.0), (3, 5, 5, 0.5), (2, 64, 64, 1.0), (7, 1000, 20, 0.8), (1, 128256, 5, 1.0),
                                      (33, 32000, 8, 1.0), (5, 50257, 20, 0.7), (300, 4096, 3, 1.0), (2, 131071, 33, 1.3),
                                      (700, 2049, 0, 1.0), (2, 1 << 20, 20, 1.0), (5000, 33, 20, 1.0),
-                                     (700, 4093, 33, 0.9)])
+                                     (700, 4093, 33, 0.9), (20, 70001, 20, 1.0), (34, 65600, 64, 0.9),
+                                     (100, 20001, 20, 1.0)])
 def test_logprobs_match_plain(dctx, src, M, V, n, T):
     rng = np.random.default_rng(M * 7 + V)
     t = _logits(rng, M, V, src)
@@ -634,11 +635,11 @@ def test_logprobs_match_plain(dctx, src, M, V, n, T):
     assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(got, again))
 
 
-@pytest.mark.parametrize("V,copies", [(20011, 1), (4001, 40)])
+@pytest.mark.parametrize("V,copies", [(20011, 1), (4001, 40), (20011, 5), (66001, 2)])
 @pytest.mark.parametrize("src", ["f32", "f16", "bf16"])
 def test_logprobs_hard_rows(dctx, src, V, copies):
     """Masked, tied, ordered and non-finite rows, each among ordinary ones; many
-    copies of them take the smaller blocks."""
+    copies of them take the smaller blocks, a few the deeper ring of clusters of 2 and 4."""
     import torch
     n = 20
     rng = np.random.default_rng(21)

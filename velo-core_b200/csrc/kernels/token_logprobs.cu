@@ -24,7 +24,7 @@
 // Measured on a B200 against 6552 GB/s: 2048 rows of 128256 f32, 20 best, 184 us back
 // to back (0.87; the stream alone 170, the rest are selections that no other block of
 // the SM hides); 576 rows of 32000 bf16, 8 best, 13.6 us (one wave of blocks: launch,
-// stream and selection in a row); one row of 128256 f32 7.9 us (latency).
+// stream and selection in a row); one row of 128256 f32 7.9 us (latency), 64 rows 11.5.
 #include <algorithm>
 #include <type_traits>
 
@@ -44,7 +44,6 @@ using sm100::smem_u32;
 
 constexpr int kErrToken = 0x6221;
 constexpr int kVecs = 4;                              // 16-byte vectors per thread and tile
-constexpr int kStages = 2;
 constexpr int kSlots = 16;                            // pieces of the row with their own maxima
 constexpr int kList = 512;                            // candidates before the bound is raised
 constexpr int kMaxCluster = 8;
@@ -55,10 +54,11 @@ constexpr int kInboxStride = kMaxTop * 8 + 16;  // sorted keys, then m, Z, Y, co
 
 // A block of kThreads and its dynamic shared memory: the ring (after the stream: the
 // candidates and the pieces to read again), the pieces' maxima, the inbox.
-template <int kThreads>
+// Two stages let four blocks share an SM.
+template <int kThreads, int kStages>
 struct Block {
     static constexpr int kWarps = kThreads / 32;
-    static constexpr int kPerSm = kThreads == 256 ? 4 : 16;
+    static constexpr int kPerSm = kThreads == 64 ? 16 : kStages == 2 ? 4 : 2;
     static constexpr int kTileVecs = kVecs * kThreads;  // 16 KB with 256 threads
     static constexpr int kRingBytes = kStages * kTileVecs * 16;
     static constexpr int kWorkOfs = (kList + kMaxTop) * 8;
@@ -195,10 +195,10 @@ struct Part {
     int first, nv, lo, hi;
 };
 
-template <typename T, int kThreads>
-__global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logprobs_kernel(const TokenLogprobsArgs a,
-                                                                                         int log_cluster) {
-    using S = Block<kThreads>;
+template <typename T, int kThreads, int kStages>
+__global__ void __launch_bounds__(kThreads, Block<kThreads, kStages>::kPerSm) token_logprobs_kernel(
+    const TokenLogprobsArgs a, int log_cluster) {
+    using S = Block<kThreads, kStages>;
     constexpr int kN = Vec<T>::n, kWarps = S::kWarps, kTileVecs = S::kTileVecs;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ Sums s_part[kWarps];
@@ -506,12 +506,22 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads>::kPerSm) token_logpr
         });
 }
 
-// Blocks per row: enough for two blocks per SM, as long as each keeps a tile's worth.
-int log_cluster_of(const TokenLogprobsArgs& a, int elt, int sm_count) {
-    const int per_tile = Block<256>::kTileVecs * 16 / elt;
+// Blocks per row: enough for `want` blocks, as long as each keeps a tile's worth.
+int log_cluster_of(const TokenLogprobsArgs& a, int elt, int want) {
+    const int per_tile = Block<256, 2>::kTileVecs * 16 / elt;
     int c = 0;
-    while (1 << c < kMaxCluster && ((long long)a.M << c) < 2LL * sm_count && a.V >> (c + 1) >= per_tile) ++c;
+    while (1 << c < kMaxCluster && ((long long)a.M << c) < want && a.V >> (c + 1) >= per_tile) ++c;
     return c;
+}
+
+template <typename T, int kStages>
+cudaError_t launch_wide(const TokenLogprobsArgs& a, int log_cluster, cudaStream_t s) {
+    static SmemAttr attr;
+    using S = Block<256, kStages>;
+    const cudaError_t e = ensure_smem(attr, token_logprobs_kernel<T, 256, kStages>, S::kSmemCluster);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(token_logprobs_kernel<T, 256, kStages>, dim3((unsigned)a.M << log_cluster), 256,
+                            log_cluster ? S::kSmemCluster : S::kSmemOne, 1 << log_cluster, s, a, log_cluster);
 }
 
 template <typename T>
@@ -519,15 +529,21 @@ cudaError_t launch_typed(const TokenLogprobsArgs& a, int sm_count, cudaStream_t 
     // many short rows: a block's time is mostly its steps of selection, so small blocks, sixteen to
     // an SM (4096 rows of 1000 f32: 40.4 us with 256 threads, 12.8 with 64)
     if ((size_t)a.V * sizeof(T) <= kShortRow && a.M > 4 * sm_count) {
-        return launch_dependent(token_logprobs_kernel<T, 64>, dim3((unsigned)a.M), 64, Block<64>::kSmemOne, 1, s, a, 0);
+        return launch_dependent(token_logprobs_kernel<T, 64, 2>, dim3((unsigned)a.M), 64, Block<64, 2>::kSmemOne, 1, s,
+                                a, 0);
     }
-    static SmemAttr attr;
-    using S = Block<256>;
-    const int log_cluster = log_cluster_of(a, (int)sizeof(T), sm_count), cluster = 1 << log_cluster;
-    cudaError_t e = ensure_smem(attr, token_logprobs_kernel<T, 256>, S::kSmemCluster);
-    if (e != cudaSuccess) return e;
-    return launch_dependent(token_logprobs_kernel<T, 256>, dim3((unsigned)a.M << log_cluster), 256,
-                            cluster > 1 ? S::kSmemCluster : S::kSmemOne, cluster, s, a, log_cluster);
+    // Rows whose clusters fill the SMs once but not twice over: one wave of blocks, each with twice the
+    // bytes in flight, against two waves' worth of blocks with the shorter ring (128256 f32 each: 19
+    // rows 11.0 -> 9.8 us, 64 rows 14.1 -> 11.5, 140 rows 21.9 -> 20.0).  With fewer blocks the longer
+    // ring is of no use (8 rows 8.5 us, 8.8 with it), with one row per block it fits less often.
+    // Clusters of 8 find two blocks' room per SM only within an SM group: past 30 or so of them a second
+    // wave forms (32 rows 13.6 us), and clusters of 4 are taken (11.1).
+    int c = log_cluster_of(a, (int)sizeof(T), sm_count);
+    if (c > 0 && a.M << c >= sm_count) {
+        if (c == 3 && (a.M << c) * 8 > 13 * sm_count) c = 2;
+        return launch_wide<T, 4>(a, c, s);
+    }
+    return launch_wide<T, 2>(a, log_cluster_of(a, (int)sizeof(T), 2 * sm_count), s);
 }
 
 }  // namespace
