@@ -291,7 +291,7 @@ typedef enum velo_elem { VELO_ELEM_F32 = 0, VELO_ELEM_F16 = 1, VELO_ELEM_BF16 = 
  *                    (VELO_KV_INT8, value = q * scale) or f32 (VELO_KV_F32)
  *   k_scale, v_scale [pool_pages][n_kv][16] f16 (INT8 only, else NULL)
  *   page_table       [rows][max_pages] u32 page ids: row b belongs to sequence b
- * head_dim 64 or 128. */
+ * head_dim 64 or 128; at most 65536 heads in these calls. */
 typedef struct velo_kv_cache {
     uint32_t struct_size;  /* sizeof(velo_kv_cache) */
     int32_t kv_dtype;      /* velo_kv_dtype */

@@ -353,6 +353,27 @@ def test_structs_of_another_size_are_refused(dctx):
     assert L.velo_cuda_decode_attention(dctx.handle, cache.ref, None, 64, None, 5000, 1, 0.0, None, None, None, 0) == bad
 
 
+def test_counts_whose_product_passes_64_bits_are_refused(dctx):
+    """4096 sequences x 2^30 heads x 2 x 2^21 pages is 2^64: the heads are refused
+    before any product is formed."""
+    import ctypes
+
+    import torch
+    z = torch.zeros(1, 1, 16, 64, device="cuda")
+    cache = velo_cuda.KvCache(z, z.clone(), torch.zeros(1, 1, dtype=torch.int32, device="cuda"))
+    L, bad = velo_cuda.lib(), velo_cuda.ERR_INVALID_ARGUMENT
+    d = velo_cuda.KvCacheDesc.from_buffer_copy(cache.desc)
+    d.max_pages = 1 << 21
+    assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(d), None, 64, None, 4096, 1 << 30, 0.0, None, None,
+                                        None, 0) == bad
+    assert "n_head" in velo_cuda.last_error()
+    d.n_kv = 1 << 30
+    assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(d), None, 64, None, 1, 1 << 30, 0.0, None, None,
+                                        None, 0) == bad
+    assert "n_kv" in velo_cuda.last_error()
+    assert L.velo_cuda_decode_attention_workspace(dctx.handle, 1 << 30, 1, 64) == 0
+
+
 # ------------------------------------------------------------------ append
 
 def _np_elem(rng, shape, src):

@@ -31,7 +31,11 @@ bool misaligned(const void* p, size_t a = 16) { return (uintptr_t)p % a != 0; }
 
 int elem_bytes(int32_t dtype) { return dtype == VELO_ELEM_F32 ? 4 : 2; }
 
-bool bad_heads(int32_t n_head, int32_t n_kv) { return n_kv < 1 || n_head < n_kv || n_head % n_kv; }
+constexpr int kMaxHeads = 1 << 16;  // products of heads, tokens and pages then stay in 64 bits
+
+bool bad_heads(int32_t n_head, int32_t n_kv) {
+    return n_kv < 1 || n_head < n_kv || n_head > kMaxHeads || n_head % n_kv;
+}
 
 int32_t check_cache(const char* op, const velo_kv_cache* k, velo::PagedKv& out) {
     if (!k) return fail(VELO_ERR_INVALID_ARGUMENT, "%s: cache is NULL", op);
@@ -42,7 +46,7 @@ int32_t check_cache(const char* op, const velo_kv_cache* k, velo::PagedKv& out) 
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: kv_dtype %d", op, k->kv_dtype);
     if (k->head_dim != 64 && k->head_dim != 128)
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: head_dim %d unsupported (64 or 128)", op, k->head_dim);
-    if (k->n_kv < 1 || k->pool_pages < 1 || k->max_pages < 0 || k->max_pages > 1 << 26)
+    if (k->n_kv < 1 || k->n_kv > kMaxHeads || k->pool_pages < 1 || k->max_pages < 0 || k->max_pages > 1 << 26)
         return fail(VELO_ERR_INVALID_ARGUMENT, "%s: n_kv %d, pool_pages %d, max_pages %d", op, k->n_kv,
                     k->pool_pages, k->max_pages);
     if (!k->k_pool || !k->v_pool || (k->max_pages > 0 && !k->page_table) ||
@@ -165,7 +169,7 @@ int32_t velo_cuda_decode_attention(velo_cuda_ctx* c, const velo_kv_cache* cache,
     if (B == 0) return VELO_OK;
     if (!q || !seq_len || !out) return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: NULL buffer");
     const int eb = cache->kv_dtype == VELO_KV_F32 ? 4 : 2;
-    if (misaligned(q) || misaligned(out) || ldq * eb % 16)
+    if (misaligned(q) || misaligned(out) || ldq * eb % 16 || misaligned(seq_len, 4) || misaligned(lse, 4))
         return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: rows must be 16-byte aligned");
     if (ldq < (int64_t)n_head * cache->head_dim)
         return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: ldq %lld below the row", (long long)ldq);
