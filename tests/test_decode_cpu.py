@@ -65,7 +65,8 @@ def _ranges(units, per_seq, main, tail, least=4, share=12, tail_units=64, tail_s
     pre = np.concatenate(([0], np.cumsum(np.asarray(units) * per_seq)))
     total = int(pre[-1])
     n = min(main, -(-total // least))
-    uncut = -(-int(np.count_nonzero(units)) * per_seq // n) * int(max(units)) - total // n <= join
+    per = -(-int(np.count_nonzero(units)) * per_seq // n)
+    uncut = 2 * (per * int(max(units)) - total // n) <= 3 * join or (per > 1 and max(units) <= 2 * join)
     if tail and total // main >= tail_units and max(units) <= tail_states * (total // share // tail):
         big, small = _Share(total - total // share, main), _Share(total // share, tail)
     else:

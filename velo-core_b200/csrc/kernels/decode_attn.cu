@@ -12,7 +12,9 @@
 // through leaves partial states (max, sum, unnormalised output) in the workspace,
 // which the join kernel, launched as a programmatic dependent, adds in order: no
 // atomics, repeatable bits.  Short items are not cut (the cut moves to their
-// start), so a batch of short contexts pays no join.
+// start), so a batch of short contexts pays no join.  What it pays is each item's start and
+// end, 1.3 us of an SM (256 x 32 tokens, 32/8 heads f16: 24.6 us), so the next item's q is on
+// its way while the warps' states of the last one are joined (29.8 without).
 //
 // A block's four warps take the units of its range in turn.  Each warp streams
 // its own units through a private ring of 8 KB (head_dim 128) stages filled by
@@ -24,10 +26,12 @@
 //  f16: K and V fragments by ldmatrix from XOR-swizzled rows.  P is split into
 //   two f16 parts (value and remainder), so that it adds no rounding of its own:
 //   with at most 8 heads the parts fill the tile's upper and lower rows.
-//  int8: fragments are read as 16 consecutive bytes per lane (the contraction
-//   order is free, q is permuted to match); K becomes f16 and V bf16, both exact;
-//   the K scale multiplies the score and the V scale the weight, in f32.  P is
-//   split into two bf16 parts, whose exponent holds any scale.
+//  int8: K fragments are 16 consecutive bytes per lane (the contraction order is free, q is
+//   permuted to match), V is transposed in 16-bit units by ldmatrix.trans.  A byte plus 128 in
+//   the low bits of an f16 is a subnormal, exact as an operand (one LOP3 or a shift and one
+//   for two values); 128 times the sum of q, and of the weights, comes off the results.  The
+//   K scale multiplies the score and the V scale the weight, which a power of two keeps in
+//   the range of the two f16 parts.
 //  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
 //   dimensions for the output.
 //
@@ -238,9 +242,13 @@ struct Cut {
 __device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int items, int longest, int join_units) {
     const int tail = plan.blocks - plan.main, blocks = min(plan.main, (total + kMinUnits - 1) / kMinUnits);
     const Share even(total, blocks);
-    // whole items make the fullest block this much longer than an equal share
-    const bool uncut =
-        total > 0 && (long long)quotient(items + blocks - 1, blocks) * longest - even.q <= join_units;
+    // Whole items make the fullest block per * longest - q longer than an equal share at most, and with
+    // several to a block half of the longest on average.  Cutting costs the join and each block an
+    // item's start and end more (128 x 100-600 tokens INT8 48.8 us cut, 45.1 uncut; where blocks would
+    // idle, 16 x 400-800, 15.5 against 17.3).
+    const int per = quotient(items + blocks - 1, blocks);
+    const bool uncut = total > 0 && (2 * ((long long)per * longest - even.q) <= 3 * join_units ||
+                                     (per > 1 && longest <= 2 * join_units));
     if (tail > 0 && quotient(total, plan.main) >= kTailUnits &&
         longest <= kTailStates * quotient(total / kTailShare, tail)) {
         const int n = total / kTailShare;
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         const Item x = item_of<kTok>(pre, lens, a.B, u);
         const int first = (u - x.start) * kTok, left = lens[x.b] - first;
         const uint32_t* row = a.kv.page_table + (size_t)x.b * a.kv.max_pages + first / kPageTokens;
-        uint4 e = make_uint4(row[0], 0, (uint32_t)(x.it / plan.tiles), left >= 32 ? ~0u : (1u << left) - 1);
+        uint4 e = make_uint4(row[0], 0, (uint32_t)(plan.tiles == 1 ? x.it : x.it / plan.tiles), left >= 32 ? ~0u : (1u << left) - 1);
         uint32_t low = kTok == 8 ? 0xffu : 0xffffu;
         e.w &= kTok == 32 ? ~0u : low;
         if (e.x >= (uint32_t)a.kv.pool_pages) {
@@ -450,19 +458,57 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
     for (int j = 0; j < S; ++j) issue(j);
 
     const float scale = a.scale * kLog2e;
+    constexpr int kH = KV == VELO_KV_F32 ? 1 : R;
+    uint32_t qb[kH][KV == VELO_KV_F32 ? 1 : D / 16][2];  // q as B fragments: head 8r + g
+    // reads an item's q; the next item's is on its way while the warps' states are joined
+    auto load_q = [&](int b, int hk, int tile) {
+        const int nh = min(kRows, plan.group - tile * kRows);
+        const Act* qp = static_cast<const Act*>(a.q) + (size_t)b * a.ldq + (size_t)(hk * plan.group + tile * kRows) * D;
+        if constexpr (KV != VELO_KV_F32) {
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int row = kPair ? g & 3 : 8 * r + g;
+                const Act* qr = qp + (size_t)row * D;
+                // the dimensions a lane holds of contraction step ks: ldmatrix's own order for f16,
+                // 4 consecutive ones for int8 (16 of four steps: two loads)
+                if constexpr (KV == VELO_KV_F16) {
+#pragma unroll
+                    for (int ks = 0; ks < D / 16; ++ks)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            qb[r][ks][i] =
+                                row < nh ? *reinterpret_cast<const uint32_t*>(qr + 16 * ks + 8 * i + 2 * t) : 0u;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+                        const uint4 v = row < nh ? *reinterpret_cast<const uint4*>(qr + 64 * (i / 2) + 16 * t + 8 * (i % 2))
+                                                 : make_uint4(0, 0, 0, 0);
+                        qb[r][2 * i][0] = v.x;
+                        qb[r][2 * i][1] = v.y;
+                        qb[r][2 * i + 1][0] = v.z;
+                        qb[r][2 * i + 1][1] = v.w;
+                    }
+                }
+            }
+        }
+    };
     int j = 0;
     int4 open = make_int4(-1, 0, 0, 0);
+    Item x{};
+    int hk = 0, tile = 0;  // of the item
+    if (u0 < u1) {
+        x = item_of<kTok>(pre, lens, a.B, u0);
+        hk = plan.tiles == 1 ? x.it : x.it / plan.tiles;
+        tile = x.it - hk * plan.tiles;
+        load_q(x.b, hk, tile);
+    }
     for (int seg = u0; seg < u1;) {
-        const Item x = item_of<kTok>(pre, lens, a.B, seg);
         const int end = x.start + x.units, seg_end = min(end, u1);
-        const int hk = x.it / plan.tiles, tile = x.it % plan.tiles;
         const int h0 = hk * plan.group + tile * kRows, nh = min(kRows, plan.group - tile * kRows);
-        const Act* qp = static_cast<const Act*>(a.q) + (size_t)x.b * a.ldq + (size_t)h0 * D;
 
         // ---- running state.  Tensor cores: scores and output are held transposed (keys or
         // dimensions x heads), so a lane has heads 8r + 2t + {0, 1}; f32: heads 2t + {0, 1} of
         // its token.  m is the reference of the weights, at most 2^8 below the largest.
-        constexpr int kH = KV == VELO_KV_F32 ? 1 : R;
         float m[kH][2], l[kH][2];
 #pragma unroll
         for (int r = 0; r < kH; ++r)
@@ -475,28 +521,21 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         float o[kH][kN][4] = {};
         constexpr int kO = KV == VELO_KV_F32 ? D / 32 : 1;      // dimensions per lane
         float of[KV == VELO_KV_F32 ? 8 : 1][kO] = {};
-        uint32_t qb[kH][KV == VELO_KV_F32 ? 1 : D / 16][2];     // q as B fragments: head 8r + g
         if constexpr (KV == VELO_KV_F32) {
+            const Act* qp = static_cast<const Act*>(a.q) + (size_t)x.b * a.ldq + (size_t)h0 * D;
             float* qs = reinterpret_cast<float*>(smem + L::kQ);
             for (int i = tid; i < 8 * D; i += kThreads) qs[i] = i / D < nh ? to_f32(qp[i]) : 0.0f;
             __syncthreads();
-        } else {
+        }
+        if constexpr (KV == VELO_KV_INT8) {  // the even, then the odd ones of 4 consecutive dimensions
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int row = kPair ? g & 3 : 8 * r + g;
-                const Act* qr = qp + (size_t)row * D;
+            for (int r = 0; r < R; ++r)
 #pragma unroll
                 for (int ks = 0; ks < D / 16; ++ks) {
-                    // the dimensions a lane holds of contraction step ks: ldmatrix's own order for
-                    // f16; the even, then the odd ones of 4 consecutive bytes for int8
-                    const int d0 = KV == VELO_KV_F16 ? 16 * ks + 2 * t : 64 * (ks / 4) + 16 * t + 4 * (ks % 4);
-                    const int d1 = d0 + (KV == VELO_KV_F16 ? 8 : 2);
-                    uint32_t x = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d0) : 0u;
-                    uint32_t y = row < nh ? *reinterpret_cast<const uint32_t*>(qr + d1) : 0u;
-                    qb[r][ks][0] = KV == VELO_KV_F16 ? x : __byte_perm(x, y, 0x5410);
-                    qb[r][ks][1] = KV == VELO_KV_F16 ? y : __byte_perm(x, y, 0x7632);
+                    const uint32_t lo = qb[r][ks][0], hi = qb[r][ks][1];
+                    qb[r][ks][0] = __byte_perm(lo, hi, 0x5410);
+                    qb[r][ks][1] = __byte_perm(lo, hi, 0x7632);
                 }
-            }
         }
         // INT8: the scores carry 128 times the sum of q, which comes off each of them.  Their f32 sums
         // are then as exact as those of a K row whose values all have its maximum's size: 2^-24 of
@@ -830,6 +869,22 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
             pending = true;
         }
 
+        Item next = x;
+        if (seg_end < u1) {
+            if (x.it + 1 < per_seq) {
+                ++next.it;
+                next.start = end;
+                if (++tile == plan.tiles) {
+                    tile = 0;
+                    ++hk;
+                }
+            } else {
+                next = item_of<kTok>(pre, lens, a.B, end);  // the next sequence's first item
+                hk = tile = 0;
+            }
+            load_q(next.b, hk, tile);
+        }
+
         // ---- the item's end in this range: the warps' states into one.  A warp's output goes
         // into the stage it has just read, which is refilled after the join.
         const uint32_t buf = stage0 + ((j + S - 1) % S) * L::kStage;  // stage of unit j - 1
@@ -844,7 +899,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                     stat_l[warp * 16 + 8 * r + 2 * t + e] = l[r][e];
                 }
             }
-        if constexpr (kPair && KV != VELO_KV_F32) {  // the remainders' columns join their heads
+        if (kPair && KV != VELO_KV_F32 && pending) {  // the remainders' columns join their heads
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
@@ -920,6 +975,7 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
         if (!whole && seg == x.start)  // begins here, ends in a later block
             open = make_int4(x.b, x.it, list.block_of(end - 1), 0);
         seg = seg_end;
+        x = next;
     }
     cp_async_wait<0>();
     if (tid == 0) desc[c] = open;
