@@ -325,10 +325,11 @@ typedef struct velo_kv_append_batch {
 
 /* Append the K/V rows of new tokens to the cache, rotated to their positions on
  * the way, and rotate their queries (RoPE of the verify step: NeoX half split,
- * llama_cpu.rs:98-132; the angles are reduced exactly, so far positions keep
- * their precision).  Asynchronous on the context stream.  f16 and f32 pages take
- * the rotated value rounded once; INT8 pages quantise it as velo_cuda_write_kv
- * does (scale = f16(max|x| / 127), truncation).  A position past the page-table
+ * llama_cpu.rs:98-132; sine and cosine of the exact angle in f32, products and
+ * sum each rounded to f32).  Asynchronous on the context stream.  f16 and f32 pages
+ * take the rotated value rounded once; INT8 pages quantise it as velo_cuda_write_kv
+ * does (scale = f16(max|x| / 127), truncation of x * (127 / max|x|)), but from f32:
+ * velo_cuda_write_kv and the verify step's commit quantise rows held in f16.  A position past the page-table
  * row, a page id outside the pool or a negative ctx_len sets the device flag
  * (velo_cuda_sync); that token's K/V are not written.  Page-table rows must not
  * share the pages written here.  Replaces kv_update / kv_update_int8

@@ -1,0 +1,69 @@
+"""The decode operators (velo_cuda_kv_append, velo_cuda_decode_attention,
+velo_cuda_token_logprobs) where a loose comparison would not see a fault: bits of
+the append, single tokens lost from long contexts, weights far below a dominant
+one, results beside a raised device flag, lengths that change between replays.
+
+Tolerances count the roundings: f16 results 2^-11 of the value (2^-25 below the
+normal range), f32 arithmetic 2^-24 per operation."""
+import numpy as np
+import pytest
+
+import velo_cuda
+from test_decode_gpu import _dev, dctx  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ append
+
+def _turned(x, cos, sin):
+    """The rotation in f32: both products and their sum rounded."""
+    h = x.shape[-1] // 2
+    a, b = x[..., :h], x[..., h:]
+    return np.concatenate((a * cos - b * sin, a * sin + b * cos), -1)
+
+
+def _append_rows(ctx, k, v, pos, D, base, kv):
+    """One token per sequence at `pos`; (pool rows [T][H][D] and scales, k and v), k_out, v_out."""
+    import torch
+    T, H = k.shape[:2]
+    width = int(pos.max()) // 16 + 1
+    table = torch.full((T, width), T + 5, dtype=torch.int32, device="cuda")
+    table[torch.arange(T, device="cuda"), _dev(pos // 16).long()] = torch.arange(T, dtype=torch.int32, device="cuda")
+    dt = {"f16": torch.float16, "int8": torch.int8, "f32": torch.float32}[kv]
+    act = torch.float32 if kv == "f32" else torch.float16
+    sc = [torch.zeros(T, H, 16, dtype=torch.float16, device="cuda") for _ in range(2)] if kv == "int8" else [None] * 2
+    cache = velo_cuda.KvCache(torch.zeros(T, H, 16, D, dtype=dt, device="cuda"),
+                              torch.zeros(T, H, 16, D, dtype=dt, device="cuda"), table, *sc)
+    ko, vo = (torch.empty(T, H, D, dtype=act, device="cuda") for _ in range(2))
+    ctx.kv_append(cache, None, _dev(k), _dev(v), _dev(pos.astype(np.int32)), None, base, k_out=ko, v_out=vo)
+    ctx.sync()
+    i, s = np.arange(T), pos % 16
+    rows = [t.cpu().numpy()[i, :, s] for t in cache.tensors[:2]]
+    scales = [None if t is None else t.cpu().numpy()[i, :, s] for t in cache.tensors[3:]]
+    return rows, scales, ko.cpu().numpy(), vo.cpu().numpy()
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16", "int8"])
+@pytest.mark.parametrize("D,base", [(128, 10000.0), (64, 500000.0)])
+def test_append_rounds_as_the_definition_says(dctx, kv, D, base):
+    """Bit for bit: f32 cosine and sine of the exact angle, both products and their
+    sum rounded to f32, then the page's rounding (INT8: 127 / max, truncation)."""
+    rng = np.random.default_rng(51)
+    T, H = 700, 3
+    k, v = rng.normal(0, 1, (2, T, H, D)).astype(np.float32)
+    pos = rng.integers(0, 120, T)
+    a = pos[:, None].astype(np.longdouble) * np.longdouble(base) ** (np.longdouble(-2) * np.arange(D // 2) / D)
+    # (each form is within 2^-46 of the exact angle: they part only that near to an f32 tie, with odds of 2^-22 an angle)
+    cos, sin = (f(a).astype(np.float32)[:, None] for f in (np.cos, np.sin))
+    rows, scales, ko, vo = _append_rows(dctx, k, v, pos, D, base, kv)
+    for x, got, sc, out in ((_turned(k, cos, sin), rows[0], scales[0], ko), (v, rows[1], scales[1], vo)):
+        if kv == "int8":
+            m = np.abs(x).max(-1)
+            assert np.array_equal(sc, (m / np.float32(127)).astype(np.float16))
+            want = np.trunc(x * (np.float32(127) / m)[..., None]).astype(np.int8)
+            assert np.array_equal(got, want)
+            assert np.array_equal(out, (want * sc.astype(np.float32)[..., None]).astype(np.float16))
+        else:
+            want = x.astype(got.dtype)
+            assert np.array_equal(got, want) and np.array_equal(out, want)

@@ -4,8 +4,10 @@
 // rot(x)_i = x_i cos a - x_{i+D/2} sin a, rot(x)_{i+D/2} = x_i sin a + x_{i+D/2} cos a,
 // a = pos * base^(-2i/D).  An angle in f32 loses all its digits far into a long
 // context (pos 10^5 leaves 2^-7 of a radian), so the frequency is kept in turns
-// as a 64-bit fraction and pos * f wraps modulo one turn by itself; only the
-// remainder in [-1/2, 1/2) turns becomes an f32.
+// as a 64-bit fraction and pos * f wraps modulo one turn by itself.  The sine and
+// cosine of the remainder are taken in 64 bits and rounded to f32; both products
+// and their sum are rounded to f32 too (no fma), so that a row, and the integers
+// an INT8 page truncates it to, have one definition whatever the compiler does.
 //
 // One block per token: its angles are computed once (a thread per pair) into
 // shared memory, then a thread takes 8 rotation pairs of a head, in equal rounds
@@ -103,9 +105,12 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
     if (ok) page = a.kv.page_table[(size_t)b * a.kv.max_pages + pi];
     if (threadIdx.x < D / 2) {
         const uint64_t turn = (uint64_t)pos * a.turns.f[threadIdx.x];
-        // the upper 32 bits as a signed fraction of a turn; sincospi takes half turns
-        const float half_turns = (float)(int32_t)(turn >> 32) * 4.656612873077393e-10f;  // 2^-31
-        sincospif(half_turns, &sn[threadIdx.x], &cs[threadIdx.x]);
+        // a signed fraction of a turn; sincospi takes half turns
+        const double half_turns = (double)(int64_t)turn * 1.0842021724855044e-19;  // 2^-63
+        double s, c;
+        sincospi(half_turns, &s, &c);
+        sn[threadIdx.x] = (float)s;
+        cs[threadIdx.x] = (float)c;
     }
     ok = ok && page < (uint32_t)a.kv.pool_pages;
     if (!ok && threadIdx.x == 0) atomicCAS(a.err, 0, kErrAppend);
@@ -123,7 +128,8 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const float c = cs[i0 + e], s = sn[i0 + e];
-                    const float y0 = x0[e] * c - x1[e] * s, y1 = x0[e] * s + x1[e] * c;
+                    const float y0 = __fsub_rn(__fmul_rn(x0[e], c), __fmul_rn(x1[e], s));
+                    const float y1 = __fadd_rn(__fmul_rn(x0[e], s), __fmul_rn(x1[e], c));
                     x0[e] = y0;
                     x1[e] = y1;
                 }
