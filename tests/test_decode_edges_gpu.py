@@ -5,11 +5,13 @@ one, results beside a raised device flag, lengths that change between replays.
 
 Tolerances count the roundings: f16 results 2^-11 of the value (2^-25 below the
 normal range), f32 arithmetic 2^-24 per operation."""
+from decimal import Decimal, getcontext
+
 import numpy as np
 import pytest
 
 import velo_cuda
-from test_decode_gpu import _dev, dctx  # noqa: F401
+from test_decode_gpu import EPS, _dev, dctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +69,32 @@ def test_append_rounds_as_the_definition_says(dctx, kv, D, base):
         else:
             want = x.astype(got.dtype)
             assert np.array_equal(got, want) and np.array_equal(out, want)
+
+
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+def test_append_angles_at_the_far_end(dctx, base):
+    """The last positions of the widest table (2^30 tokens): rows of (1, 0) become
+    the f32 cosine and sine of the exact angle, whose turns are off by 2^-64 a position."""
+    import torch
+    D, width = 64, 1 << 26
+    getcontext().prec = 60
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    pos = np.asarray([16 * width - 1, 16 * width - 12345, 777777777])
+    table = torch.full((1, width), 9, dtype=torch.int32, device="cuda")
+    for i, p in enumerate(pos):
+        table[0, int(p) // 16] = i
+    z = torch.zeros(3, 1, 16, D, device="cuda")
+    cache = velo_cuda.KvCache(z, z.clone(), table)
+    k = torch.zeros(1, 1, D, device="cuda")
+    k[..., :D // 2] = 1
+    for i, p in enumerate(pos):
+        dctx.kv_append(cache, None, k, k, torch.tensor([int(p)], dtype=torch.int32, device="cuda"), None, base)
+    dctx.sync()
+    got = cache.tensors[0].cpu().numpy()
+    for i, p in enumerate(pos):
+        for e in range(D // 2):
+            a = Decimal(int(p)) * (Decimal(base).ln() * Decimal(-2 * e) / Decimal(D)).exp() / (2 * pi)  # turns
+            a = float(2 * pi * (a - a.to_integral_value()))
+            for have, want in ((got[i, 0, p % 16, e], np.cos(a)), (got[i, 0, p % 16, D // 2 + e], np.sin(a))):
+                # half a step of f32, 2^30 x 2^-64 turns of 2 pi, the 64-bit forms' own rounding
+                assert abs(have - want) <= abs(want) * EPS + 2.0 ** -31 + 2.0 ** -50, (p, e)

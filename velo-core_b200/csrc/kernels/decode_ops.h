@@ -22,8 +22,8 @@ struct PagedKv {
 };
 
 // base^(-2i/D) / 2pi of every rotation pair, in turns: 64-bit binary fractions,
-// so that position x frequency modulo one turn is one wrapping multiplication
-// and exact to 2^-64 turns per position.
+// so that position x frequency modulo one turn is one wrapping multiplication,
+// off by no more than 2^-64 turns per position.
 struct RopeTurns {
     uint64_t f[64];
 };

@@ -71,10 +71,11 @@ int32_t check_cache(const char* op, const velo_kv_cache* k, velo::PagedKv& out) 
 // The rotation table of (base, head_dim); the context keeps the last one.
 const velo::RopeTurns& rope_turns(velo_cuda_ctx* c, float base, int D) {
     if (c->rope_base != base || c->rope_dim != D) {
-        const double two_pi = 6.283185307179586476925286766559;
+        // (the extended type's 64-bit mantissa: a double would leave 2^-56 turns per position)
+        const long double two_pi = 6.283185307179586476925286766559L;
         for (int i = 0; i < D / 2; ++i)
             c->rope_turns[i] =
-                (uint64_t)std::floor(std::ldexp(std::pow((double)base, -2.0 * i / D) / two_pi, 64) + 0.5);
+                (uint64_t)std::floor(std::ldexp(std::pow((long double)base, -2.0L * i / D) / two_pi, 64) + 0.5L);
         c->rope_base = base;
         c->rope_dim = D;
     }
