@@ -309,8 +309,8 @@ typedef struct velo_kv_append_batch {
     const void *k, *v;        /* [n_tokens][n_kv][head_dim] */
     int64_t ldq, ldk, ldv;    /* token t's row starts at t * ld elements, so that all three may be
                                  slices of one projection's output; rows 16-byte aligned */
-    const int32_t *seq_start; /* [B+1], non-decreasing: tokens seq_start[b] .. seq_start[b+1] - 1
-                                 continue sequence b; rows from seq_start[B] on are padding, for
+    const int32_t *seq_start; /* [B+1], from 0, non-decreasing, n_tokens at most: tokens seq_start[b] ..
+                                 seq_start[b+1] - 1 continue sequence b; rows from seq_start[B] on are padding, for
                                  which nothing is read or written.  NULL: token t is sequence t's
                                  only one (n_tokens == B) */
     const int32_t *ctx_len;   /* [B] tokens cached before the call: token t of sequence b goes to
@@ -329,10 +329,12 @@ typedef struct velo_kv_append_batch {
  * sum each rounded to f32).  Asynchronous on the context stream.  f16 and f32 pages
  * take the rotated value rounded once; INT8 pages quantise it as velo_cuda_write_kv
  * does (scale = f16(max|x| / 127), truncation of x * (127 / max|x|)), but from f32:
- * velo_cuda_write_kv and the verify step's commit quantise rows held in f16.  A position past the page-table
- * row, a page id outside the pool or a negative ctx_len sets the device flag
- * (velo_cuda_sync); that token's K/V are not written.  Page-table rows must not
- * share the pages written here.  Replaces kv_update / kv_update_int8
+ * velo_cuda_write_kv and the verify step's commit quantise rows held in f16.  A
+ * position past the page-table row, a page id outside the pool or a negative
+ * ctx_len sets the device flag (velo_cuda_sync); that token's K/V are not written.
+ * Starts that are not as seq_start asks set the flag too, and which tokens are
+ * then written is open (never outside the sequences' pages).  Page-table rows
+ * must not share the pages written here.  Replaces kv_update / kv_update_int8
  * (src/kernels.metal:619-645, 753-802) after the per-head rope of forward_one
  * (src/llama_cpu.rs:113-132). */
 VELO_API int32_t velo_cuda_kv_append(velo_cuda_ctx *ctx, const velo_kv_cache *cache,

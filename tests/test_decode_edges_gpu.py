@@ -98,3 +98,30 @@ def test_append_angles_at_the_far_end(dctx, base):
             for have, want in ((got[i, 0, p % 16, e], np.cos(a)), (got[i, 0, p % 16, D // 2 + e], np.sin(a))):
                 # half a step of f32, 2^30 x 2^-64 turns of 2 pi, the 64-bit forms' own rounding
                 assert abs(have - want) <= abs(want) * EPS + 2.0 ** -31 + 2.0 ** -50, (p, e)
+
+
+@pytest.mark.parametrize("B", [3, 300])
+def test_append_flags_starts_that_lose_or_move_tokens(dctx, B):
+    """Starts past n_tokens, not from 0, falling or negative set the device flag, with
+    a sequence per thread (B = 3) and with the search (B = 300); good ones do not."""
+    import torch
+    k = torch.ones(B, 1, 64, device="cuda")
+    n = torch.full((B,), 3, dtype=torch.int32, device="cuda")
+    z = torch.zeros(B, 1, 16, 64, device="cuda")
+    cache = velo_cuda.KvCache(z, z.clone(), torch.arange(B, dtype=torch.int32, device="cuda").view(B, 1))
+    good = np.arange(B + 1, dtype=np.int32)
+
+    def run(start):
+        dctx.kv_append(cache, None, k, k, n, None, 10000.0, seq_start=_dev(start))
+        dctx.sync()
+    bad = [np.append(good[:-1], B + 1), np.append(good[:-1], 2 ** 31 - 1), np.append([-2], good[1:]), np.append([1], good[1:]),
+           good - 2, np.append(good[:-1], -1), np.append(good[:-1], 0)]
+    bad.append(good.copy())
+    bad[-1][2] = 0  # 0, 1, 0, 3: falls and rises again
+    for start in bad:
+        with pytest.raises(velo_cuda.VeloError) as e:
+            run(start.astype(np.int32))
+        assert e.value.status == velo_cuda.ERR_DEVICE_FLAG
+    short = np.minimum(good, B - 2)  # padding behind, an empty sequence at the end
+    for start in (good, short, np.zeros(B + 1, np.int32)):
+        run(start.astype(np.int32))

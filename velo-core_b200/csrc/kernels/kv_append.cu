@@ -48,6 +48,12 @@ __device__ __forceinline__ int find_sequence(const int32_t* start, int B, int t)
     return lo;
 }
 
+// Sequence i's tokens [begin, end): the first block looks at all of them.  Starts that
+// do not rise from 0 to n_tokens at most would leave tokens out or move them.
+__device__ __forceinline__ void check_start(const KvAppendArgs& a, int i, int begin, int end) {
+    if (i < a.B && ((i == 0 && begin != 0) || end < begin || end > a.T)) atomicCAS(a.err, 0, kErrAppend);
+}
+
 // This thread's 8 rotation pairs of head `hh` (q heads, then k, then v) of token t.
 template <typename In, int D>
 __device__ __forceinline__ const In* source(const KvAppendArgs& a, int t, int hh, int i0) {
@@ -71,6 +77,7 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
     } else if (a.B <= (int)blockDim.x) {  // a thread per sequence: one round of reads
         const int i = threadIdx.x, total = a.seq_start[a.B];
         const int begin = i < a.B ? a.seq_start[i] : 0, end = i < a.B ? a.seq_start[i + 1] : 0;
+        if (t == 0) check_start(a, i, begin, end);
         if (t >= total) return;  // padding rows
         const int len = i < a.B ? a.ctx_len[i] : 0;
         const bool here = i < a.B && begin <= t && t < end;
@@ -86,6 +93,8 @@ __global__ void __launch_bounds__(kMaxThreads, kMinBlocks) kv_append_kernel(cons
             cached = s_seq[2];
         }
     } else {
+        if (t == 0)
+            for (int i = threadIdx.x; i < a.B; i += blockDim.x) check_start(a, i, a.seq_start[i], a.seq_start[i + 1]);
         if (t >= a.seq_start[a.B]) return;
         b = find_sequence(a.seq_start, a.B, t);
         if (b >= 0) {
