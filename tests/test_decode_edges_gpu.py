@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 import velo_cuda
-from test_decode_gpu import EPS, _dev, dctx  # noqa: F401
+from test_decode_gpu import ATTN, EPS, _attend, _cache, _dev, _half_step, dctx  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +125,132 @@ def test_append_flags_starts_that_lose_or_move_tokens(dctx, B):
     short = np.minimum(good, B - 2)  # padding behind, an empty sequence at the end
     for start in (good, short, np.zeros(B + 1, np.int32)):
         run(start.astype(np.int32))
+
+
+# ------------------------------------------------------------------ attention
+
+TOKENS = {"f16": 16, "int8": 32, "f32": 8}  # of a step
+
+
+def _exact(q, d, lens, kv, scale=None):
+    """64-bit attention per head with what its rounding is measured by: out, lse,
+    sum p |v| (INT8: and sum p 255 |scale|, whose values carry a bias of 128 through
+    the sums), the largest |v|, and the largest sum of a score's |products|."""
+    B, Hq, D = q.shape
+    Hkv = d["k"].shape[1]
+    scale = 1.0 / np.sqrt(D) if scale is None else scale
+    out, mag = np.zeros((2, B, Hq, D))
+    lse, reach, mag8, vmax = np.full((B, Hq), -np.inf), *np.zeros((3, B, Hq))
+    for b in range(B):
+        n = int(lens[b])
+        if n == 0:
+            continue
+        ids = d["table"][b, :-(-n // 16)].astype(np.int64)
+
+        def rows(name):
+            x = d[name][ids].astype(np.float64).transpose(1, 0, 2, 3).reshape(Hkv, -1, D)[:, :n]
+            if kv != "int8":
+                return x, None
+            sc = d[name + "_scale"][ids].astype(np.float64).transpose(1, 0, 2).reshape(Hkv, -1)[:, :n]
+            return x * sc[..., None], sc
+        (k, ks), (v, vs) = rows("k"), rows("v")
+        for h in range(Hq):
+            g = h // (Hq // Hkv)
+            qh = q[b, h].astype(np.float64) * scale
+            x = k[g] @ qh
+            reach[b, h] = (np.abs(k[g]) @ np.abs(qh)).max() if kv != "int8" else 255 * np.abs(ks[g]).max() * np.abs(qh).sum()
+            m = x.max()
+            e = np.exp(x - m)
+            lse[b, h] = m + np.log(e.sum())
+            w = e / e.sum()
+            out[b, h], mag[b, h], vmax[b, h] = w @ v[g], w @ np.abs(v[g]), np.abs(v[g]).max()
+            if kv == "int8":
+                mag8[b, h] = 255 * (w @ np.abs(vs[g]))
+    return out, lse, mag, mag8, vmax, reach
+
+
+def _check_close(out, lse, q, d, lens, kv, scale=None):
+    """Tolerances per sequence and head.  A score: D products added in f32 (INT8: D / 16
+    matrix steps of 2^-22 of the biased sum), the change of base and the difference from
+    the reference, 2^-22 of its size.  A weight: that, its exponential 2^-21, its two f16
+    parts 2^-21.  The weighted sums: 2^-23 per addition of a chain through one warp's steps
+    of the item, 32 tokens within a step and 64 states joined; INT8's six products of
+    biased values a step.  f16 parts below the normal range: 2^-39 of a step's largest
+    weight for each of 32 tokens.  f16 output: half a step."""
+    want, want_lse, mag, mag8, vmax, reach = _exact(q, d, lens, kv, scale)
+    Hkv, D = d["k"].shape[1], q.shape[-1]
+    units = -(-np.asarray(lens, np.int64) // TOKENS[kv])
+    chain = np.minimum(units / 4 + 1, units.sum() * Hkv * -(-(q.shape[1] // Hkv) // 4) / 296 + 8) + 96
+    ds = reach * ((D / 16 + 8) * 2.0 ** -22 if kv == "int8" else (D + 8) * EPS) + 2.0 ** -22 * np.abs(reach)
+    dw = ds + 2.0 ** -20 + chain[:, None] * 2.0 ** -23
+    tol = _half_step(want, kv != "f32") + 2 * dw[..., None] * mag
+    if kv != "f32":
+        tol += (2.0 ** -20 * mag8 + 2.0 ** -34 * vmax)[..., None]
+    assert np.isfinite(out).all()
+    err = np.abs(out - want)
+    assert (err <= tol).all(), ((err / tol).max(), np.unravel_index((err / tol).argmax(), err.shape))
+    if lse is not None:
+        empty = np.isneginf(want_lse)
+        assert (lse[empty] == want_lse[empty]).all()
+        err = np.abs(lse - want_lse)[~empty]
+        assert (err <= (dw + 4 * EPS * (1 + np.abs(want_lse)))[~empty]).all()
+
+
+def _set(d, kv, b, t, name, row, scale=None):
+    """Token t of sequence b: `row` for every KV head."""
+    at = d["table"][b, t // 16], slice(None), t % 16
+    d[name][at] = row
+    if kv == "int8":
+        d[name + "_scale"][at] = scale
+
+
+@pytest.mark.parametrize("group", [4, 8, 16])
+@pytest.mark.parametrize("kv,n,nats", [("f16", 203, 18), ("f16", 4095, 18.5), ("f16", 30000, 12), ("f16", 30000, 16),
+                                       ("f16", 30000, 20), ("f16", 100003, 23), ("int8", 203, 18), ("int8", 4095, 21),
+                                       ("int8", 30000, 16), ("int8", 30000, 23), ("f32", 4095, 18.5)])
+def test_attention_small_weights_beside_a_dominant_one(dctx, kv, n, nats, group):
+    """One token takes nearly all of the weight and has a V of 0: the output is what the
+    others, `nats` below it, add up to, and keeps its digits."""
+    rng = np.random.default_rng(int(n + 10 * nats))
+    D, Hkv, lens = 64, 2, [n, 40]
+    d = _cache(rng, kv, lens, Hkv, D)
+    for b, m in enumerate(lens):
+        low = -nats * (1 + 0.02 * rng.random((m, 1)))
+        ids, slots = d["table"][b, np.arange(m) // 16], np.arange(m) % 16
+        v = 1 + rng.normal(0, 0.5, (m, Hkv, D))
+        if kv == "int8":
+            d["k"][ids, :, slots] = 0
+            d["k"][ids, :, slots, 0] = -127
+            d["k_scale"][ids, :, slots] = (-low / 127).astype(np.float16)
+            d["v"][ids, :, slots] = np.clip(np.trunc(v * 40), -127, 127)
+            d["v_scale"][ids, :, slots] = 0.025
+        else:
+            d["k"][ids, :, slots] = 0
+            d["k"][ids, :, slots, 0] = low
+            d["v"][ids, :, slots] = v
+        _set(d, kv, b, int(m * 0.37), "k", 0, 0.1)
+        _set(d, kv, b, int(m * 0.37), "v", 0, 0.0)
+    q = np.zeros((2, group * Hkv, D), np.float32 if kv == "f32" else np.float16)
+    q[:, :, 0] = 1 + 0.02 * np.arange(group * Hkv) / group
+    out, lse = _attend(dctx, d, q, lens, scale=1.0)
+    _check_close(out, lse, q, d, lens, kv, 1.0)
+
+
+def test_attention_int8_scale_of_a_token_without_weight(dctx):
+    """A V scale 2^25 above the others', on a token 60 nats below them: it costs them no digits."""
+    rng = np.random.default_rng(61)
+    lens, Hkv, D = [700, 33], 2, 128
+    d = _cache(rng, "int8", lens, Hkv, D)
+    for name in ("k", "v"):
+        d[name + "_scale"][:] = np.where(np.isfinite(d[name + "_scale"]), np.float16(0.001), d[name + "_scale"])
+    q = np.zeros((2, 16, D), np.float16)
+    q[:, :, 0] = 1
+    for b, t in ((0, 5), (0, 350), (1, 9)):
+        row = np.zeros(D)
+        row[0] = -127
+        _set(d, "int8", b, t, "k", row, 0.5)
+        _set(d, "int8", b, t, "v", 127, 60000)
+    out, lse = _attend(dctx, d, q, lens, scale=1.0)
+    # (the token's own e^-63.5 x 127 x 60000 is below 2^-60: vmax is the others')
+    keep = dict(d, v_scale=np.where(d["v_scale"] == 60000, np.float16(0), d["v_scale"]))
+    _check_close(out, lse, q, keep, lens, "int8", 1.0)

@@ -20,20 +20,23 @@
 // its own units through a private ring of 8 KB (head_dim 128) stages filled by
 // 16-byte cp.async (three stages: 96 KB in flight per block), so no block-wide
 // barrier stands between the loads and the arithmetic; tokens past the length are
-// zero-filled, never read.  Query heads of a KV head are the rows of mma.sync
+// zero-filled, never read.  Query heads of a KV head are the columns of mma.sync
 // tiles (m16n8k16; tcgen05's 128-row tiles would be 1/16 full at 8 heads a KV head).
 //
-//  f16: K and V fragments by ldmatrix from XOR-swizzled rows.  P is split into
-//   two f16 parts (value and remainder), so that it adds no rounding of its own:
-//   with at most 8 heads the parts fill the tile's upper and lower rows.
+//  The weights are held in f32 and enter P V as two f16 parts (value and remainder) in a
+//   unit of the step's own largest weight of that head: 2^-22 of a weight, or 2^-39 of the
+//   step's largest, is all that is lost, so many small weights beside a dominant one add up
+//   as the f32 sum in the denominator does.  (In units of the reference, a weight 2^-25
+//   below it would be 0.)  The step's sums are added to the output by f32 multiply-adds.
+//   With at most 4 heads the parts share a tile: columns 0 - 3 and 4 - 7.
+//  f16: K and V fragments by ldmatrix from XOR-swizzled rows.
 //  int8: K fragments are 16 consecutive bytes per lane (the contraction order is free, q is
 //   permuted to match), V is transposed in 16-bit units by ldmatrix.trans.  A byte plus 128 in
 //   the low bits of an f16 is a subnormal, exact as an operand (one LOP3 or a shift and one
 //   for two values); 128 times the sum of q, and of the weights, comes off the results.  The
-//   K scale multiplies the score and the V scale the weight, which a power of two keeps in
-//   the range of the two f16 parts.
+//   K scale multiplies the score and the V scale the weight.
 //  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
-//   dimensions for the output.
+//   dimensions for the output.  (Exponentials are ex2.approx, 2^-22, in all forms.)
 //
 // Measured on a B200 against 6552 GB/s: 64 sequences of 3900 - 4290 f16 tokens, 64/8
 // heads, 168 us back to back (0.98); one of 100003 tokens 73 us (0.86: start-up and
@@ -155,6 +158,18 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], const uint32_t (&a)[
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                             const float (&c)[4]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// The largest over the lanes of a head's scores (those with the same lane % 4).
+__device__ __forceinline__ float max_of_tokens(float x) {
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+    return x;
 }
 
 // Two f32 as a pair of 16-bit parts and the pair of their remainders.
@@ -558,9 +573,6 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                 for (int e = 0; e < 2; ++e) q128[r][e] = 128.0f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + e));
             }
         }
-        // INT8: the weights times the V scales are kept within f16 by a power of two that brings
-        // the largest scale seen to 2^5 .. 2^6 (0: none yet)
-        float v_unit = 0.0f;
         bool pending = false;
         for (; j < n_w && u0 + warp + kWarps * j < seg_end; ++j) {
             if (pending) issue(j - 1 + S);
@@ -645,29 +657,20 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                                 x = (KV == VELO_KV_INT8 ? fmaf(x, 16777216.0f, -q128[r][e]) : x) * f;
                             }
                     }
-                // the largest scores and V scale of the step
-                float top[R][2], big = 0.0f;
-                auto largest = [&] {
+                // one rarely taken branch: a ragged step or a new reference
+                bool adjust = present != kFull;
+                float top[R][2];
+                auto largest = [&] {  // of this lane's scores
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            float mx = fmaxf(s[0][r][e], s[0][r][2 + e]);
+                            top[r][e] = fmaxf(s[0][r][e], s[0][r][2 + e]);
 #pragma unroll
-                            for (int kt = 1; kt < kT; ++kt) mx = fmaxf(mx, fmaxf(s[kt][r][e], s[kt][r][2 + e]));
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                            top[r][e] = mx;
+                            for (int kt = 1; kt < kT; ++kt) top[r][e] = fmaxf(top[r][e], fmaxf(s[kt][r][e], s[kt][r][2 + e]));
                         }
-                    if constexpr (KV == VELO_KV_INT8) {
-                        big = fmaxf(fmaxf(fabsf(vs[0][0]), fabsf(vs[0][1])), fmaxf(fabsf(vs[1][0]), fabsf(vs[1][1])));
-#pragma unroll
-                        for (int d = 4; d < 32; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
-                    }
                 };
                 largest();
-                // one rarely taken branch: a ragged step, a new reference, a new unit of the V scales
-                bool adjust = present != kFull || (KV == VELO_KV_INT8 && !(big * v_unit <= 64.0f && v_unit > 0.0f));
 #pragma unroll
                 for (int r = 0; r < R; ++r) adjust |= top[r][0] > m[r][0] + 8.0f || top[r][1] > m[r][1] + 8.0f;
                 if (__any_sync(0xffffffffu, adjust)) {
@@ -683,114 +686,146 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                                 }
                         largest();
                     }
-                    float f = 1.0f;
-                    if (KV == VELO_KV_INT8 && !(big * v_unit <= 64.0f && v_unit > 0.0f)) {
-                        // 2^5 / the power of two below the largest scale (f16: at least 2^-24)
-                        const float unit = big > 0.0f ? __uint_as_float(((254u + 5u) << 23) - (__float_as_uint(big) & 0x7f800000u)) : 0.0f;
-                        f = v_unit > 0.0f ? unit / v_unit : 0.0f;
-                        v_unit = unit;
-                    }
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float mn = fmaxf(m[r][e], top[r][e]);
+                            const float mn = fmaxf(m[r][e], max_of_tokens(top[r][e]));
                             const float alpha = mn == m[r][e] ? 1.0f : ex2_approx(m[r][e] - mn);
                             m[r][e] = mn;
                             l[r][e] *= alpha;
 #pragma unroll
                             for (int n = 0; n < kN; ++n) {
-                                o[r][n][e] *= alpha * f;
-                                o[r][n][2 + e] *= alpha * f;
+                                o[r][n][e] *= alpha;
+                                o[r][n][2 + e] *= alpha;
                             }
                         }
                 }
-                if constexpr (KV == VELO_KV_INT8) {
+                // ---- the weights in f32, for P V times the V scale, and each head's unit: the power of two
+                // that brings the step's largest to 2^14 .. 2^15, so that the two f16 parts keep 2^-22 of a
+                // weight, or 2^-39 of the step's largest one, however far below the reference all of them are
+                float unit[R][2];  // then what undoes it (and, INT8, the values' 2^-24)
+                {
+                    float most[R][2] = {};
 #pragma unroll
                     for (int kt = 0; kt < kT; ++kt)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) vs[kt][i] *= v_unit;
+                        for (int r = 0; r < R; ++r)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    float& x = s[kt][r][2 * i + e];
+                                    x = ex2_approx(x - (m[r][e] == -INFINITY ? 0.0f : m[r][e]));
+                                    l[r][e] += x;
+                                    if constexpr (KV == VELO_KV_INT8) x *= vs[kt][i];
+                                    most[r][e] = fmaxf(most[r][e], KV == VELO_KV_INT8 ? fabsf(x) : x);
+                                }
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t up = min(268u - (__float_as_uint(max_of_tokens(most[r][e])) >> 23), 254u);
+                            const float by = __uint_as_float(up << 23);
+#pragma unroll
+                            for (int kt = 0; kt < kT; ++kt) {
+                                s[kt][r][e] *= by;
+                                s[kt][r][2 + e] *= by;
+                            }
+                            unit[r][e] = __uint_as_float((254u - up + (KV == VELO_KV_INT8 ? 24u : 0u)) << 23);
+                        }
                 }
                 // ---- the weights, as value and remainder, become B fragments by transposition; P V
-                float bias[R][4];
+                uint32_t hi[kT][R][2], lo[kT][R][2];  // kPair: hi has both
 #pragma unroll
-                for (int kt = 0; kt < kT; ++kt) {
-                    uint32_t hi[R][2], lo[R][2];  // kPair: hi has both
+                for (int kt = 0; kt < kT; ++kt)
 #pragma unroll
                     for (int r = 0; r < R; ++r)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float r0 = m[r][0] == -INFINITY ? 0.0f : m[r][0], r1 = m[r][1] == -INFINITY ? 0.0f : m[r][1];
-                            const float p0 = ex2_approx(s[kt][r][2 * i] - r0), p1 = ex2_approx(s[kt][r][2 * i + 1] - r1);
-                            l[r][0] += p0;
-                            l[r][1] += p1;
-                            const float v = KV == VELO_KV_INT8 ? vs[kt][i] : 1.0f;
-                            split_f16(p0 * v, p1 * v, hi[r][i], lo[r][i]);
+                            uint32_t h, rest;
+                            split_f16(s[kt][r][2 * i], s[kt][r][2 * i + 1], h, rest);
                             if constexpr (kPair) {
-                                hi[r][i] = transpose8x8(t < 2 ? hi[r][i] : lo[r][i]);
+                                hi[kt][r][i] = transpose8x8(t < 2 ? h : rest);
                             } else {
-                                hi[r][i] = transpose8x8(hi[r][i]);
-                                lo[r][i] = transpose8x8(lo[r][i]);
+                                hi[kt][r][i] = transpose8x8(h);
+                                lo[kt][r][i] = transpose8x8(rest);
                             }
                         }
-                    const int r8 = lane & 7, mi = lane >> 3, row = kt * 16 + (mi >> 1) * 8 + r8;
-                    const uint32_t vb = st + L::kHalf + row * L::kRow, flip = v_swizzle(row);
-                    if constexpr (KV == VELO_KV_F16) {
+                auto add_tile = [&](float (&to)[4], const float (&y)[4], int r) {
 #pragma unroll
-                        for (int n = 0; n < kN; ++n) {
-                            uint32_t vf[4];
-                            ldmatrix_x4_trans(vf, vb + (((2 * n + (mi & 1)) ^ flip) << 4));
+                    for (int e = 0; e < 4; e += 2) {
+                        const float2 x = __ffma2_rn(make_float2(y[e], y[e + 1]), make_float2(unit[r][0], unit[r][1]),
+                                                    make_float2(to[e], to[e + 1]));
+                        to[e] = x.x;
+                        to[e + 1] = x.y;
+                    }
+                };
+                const int r8 = lane & 7, mi = lane >> 3, row0 = (mi >> 1) * 8 + r8;
+                if constexpr (KV == VELO_KV_F16) {
+                    const uint32_t vb = st + L::kHalf + row0 * L::kRow, flip = v_swizzle(row0);
 #pragma unroll
-                            for (int r = 0; r < R; ++r) {
-                                mma_f16(o[r][n], vf, hi[r][0], hi[r][1]);
-                                if constexpr (!kPair) mma_f16(o[r][n], vf, lo[r][0], lo[r][1]);
-                            }
+                    for (int n = 0; n < kN; ++n) {
+                        uint32_t vf[4];
+                        ldmatrix_x4_trans(vf, vb + (((2 * n + (mi & 1)) ^ flip) << 4));
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            float y[4];
+                            mma_f16_zero(y, vf, hi[0][r][0], hi[0][r][1]);
+                            if constexpr (!kPair) mma_f16(y, vf, lo[0][r][0], lo[0][r][1]);
+                            add_tile(o[r][n], y, r);
                         }
-                    } else {
-                        // minus 128 times the weights, as the same products: what the step's outputs carry too much
-                        const uint32_t minus128[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+                    }
+                } else {
+                    // the step's sums start from minus 128 times its weights, as the same products: what
+                    // its values carry too much, never more than the step's own weights
+                    const uint32_t minus128[4] = {0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u};
+                    float bias[R][4];
+#pragma unroll
+                    for (int kt = 0; kt < kT; ++kt)
 #pragma unroll
                         for (int r = 0; r < R; ++r) {
                             if (kt == 0)
-                                mma_f16_zero(bias[r], minus128, hi[r][0], hi[r][1]);
+                                mma_f16_zero(bias[r], minus128, hi[kt][r][0], hi[kt][r][1]);
                             else
-                                mma_f16(bias[r], minus128, hi[r][0], hi[r][1]);
-                            if constexpr (!kPair) mma_f16(bias[r], minus128, lo[r][0], lo[r][1]);
+                                mma_f16(bias[r], minus128, hi[kt][r][0], hi[kt][r][1]);
+                            if constexpr (!kPair) mma_f16(bias[r], minus128, lo[kt][r][0], lo[kt][r][1]);
                         }
-                        // transposed as 16-bit units, a register holds two dimensions of two tokens:
-                        // row 8 half + g of tile n is dimension 32 (n / 2) + 16 half + 2 g + n % 2
+                    // transposed as 16-bit units, a register holds two dimensions of two tokens:
+                    // row 8 half + g of tile n is dimension 32 (n / 2) + 16 half + 2 g + n % 2
 #pragma unroll
-                        for (int n = 0; n < kN; n += 2) {
+                    for (int n = 0; n < kN; n += 2) {
+                        float y[2][R][4];
+#pragma unroll
+                        for (int kt = 0; kt < kT; ++kt) {
+                            const int row = kt * 16 + row0;
                             uint32_t w[4];
-                            ldmatrix_x4_trans(w, vb + (((n + (mi & 1)) ^ flip) << 4));
+                            ldmatrix_x4_trans(w, st + L::kHalf + row * L::kRow + (((n + (mi & 1)) ^ v_swizzle(row)) << 4));
                             const uint32_t va[4] = {even_bytes(w[0]), even_bytes(w[1]), even_bytes(w[2]),
                                                     even_bytes(w[3])};
                             const uint32_t vo[4] = {odd_bytes(w[0]), odd_bytes(w[1]), odd_bytes(w[2]),
                                                     odd_bytes(w[3])};
 #pragma unroll
                             for (int r = 0; r < R; ++r) {
-                                mma_f16(o[r][n], va, hi[r][0], hi[r][1]);
-                                mma_f16(o[r][n + 1], vo, hi[r][0], hi[r][1]);
+                                if (kt == 0) {
+                                    mma_f16_from(y[0][r], va, hi[kt][r][0], hi[kt][r][1], bias[r]);
+                                    mma_f16_from(y[1][r], vo, hi[kt][r][0], hi[kt][r][1], bias[r]);
+                                } else {
+                                    mma_f16(y[0][r], va, hi[kt][r][0], hi[kt][r][1]);
+                                    mma_f16(y[1][r], vo, hi[kt][r][0], hi[kt][r][1]);
+                                }
                                 if constexpr (!kPair) {
-                                    mma_f16(o[r][n], va, lo[r][0], lo[r][1]);
-                                    mma_f16(o[r][n + 1], vo, lo[r][0], lo[r][1]);
+                                    mma_f16(y[0][r], va, lo[kt][r][0], lo[kt][r][1]);
+                                    mma_f16(y[1][r], vo, lo[kt][r][0], lo[kt][r][1]);
                                 }
                             }
                         }
+#pragma unroll
+                        for (int r = 0; r < R; ++r) {
+                            add_tile(o[r][n], y[0][r], r);
+                            add_tile(o[r][n + 1], y[1][r], r);
+                        }
                     }
-                }
-                if constexpr (KV == VELO_KV_INT8) {
-                    // taken off after every step, the bias never outgrows a step's own weights in the sums
-#pragma unroll
-                    for (int r = 0; r < R; ++r)
-#pragma unroll
-                        for (int n = 0; n < kN; ++n)
-#pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                const float2 x = __fadd2_rn(make_float2(o[r][n][e], o[r][n][e + 1]), make_float2(bias[r][0], bias[r][1]));
-                                o[r][n][e] = x.x;
-                                o[r][n][e + 1] = x.y;
-                            }
                 }
             } else {
                 // ---- f32 scores: token g, dimensions 16 i + 4 t .. + 3 of every head
@@ -915,15 +950,13 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(KV, kTiles)) decode_at
                     for (int e = 0; e < kO; ++e) dst[h * D + lane * kO + e] = of[h][e];
             } else {
                 // [head][fragment row], eights XORed with the head against bank conflicts
-                const float unscale = v_unit > 0.0f ? 16777216.0f / v_unit : 0.0f;
 #pragma unroll
                 for (int r = 0; r < R; ++r)
 #pragma unroll
                     for (int n = 0; n < kN; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (!kPair || t < 2) dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] =
-                                KV == VELO_KV_INT8 ? o[r][n][e] * unscale : o[r][n][e];
+                            if (!kPair || t < 2) dst[(8 * r + 2 * t + (e & 1)) * D + ((16 * n + 8 * (e >> 1) + g) ^ (t << 3))] = o[r][n][e];
             }
         }
         __syncthreads();
