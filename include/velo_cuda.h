@@ -362,7 +362,9 @@ VELO_API size_t velo_cuda_decode_attention_workspace(velo_cuda_ctx *ctx, int32_t
  * h / (n_head / n_kv).  Slots past seq_len in the last page are never used,
  * whatever they hold.  A negative or too long seq_len (clamped to the
  * page-table row) and a page id outside the pool (its tokens are left out) set
- * the device flag (velo_cuda_sync).  B <= 4096.  Repeated calls give the same
+ * the device flag (velo_cuda_sync).  B <= 4096, and B x n_kv x max_pages x
+ * ceil(n_head / n_kv / 16) x 1 (f16 pages), 1/2 (INT8, the pages rounded up to two)
+ * or, with 8 in place of 16, 2 (f32) is 2^30 at most.  Repeated calls give the same
  * bits.  Replaces paged_attention_flash (src/kernels.metal:440-501, 672-732);
  * velo_cuda_tree_attention serves draft trees. */
 VELO_API int32_t velo_cuda_decode_attention(velo_cuda_ctx *ctx, const velo_kv_cache *cache, const void *q,

@@ -192,7 +192,7 @@ def _check_close(out, lse, q, d, lens, kv, scale=None):
     if lse is not None:
         empty = np.isneginf(want_lse)
         assert (lse[empty] == want_lse[empty]).all()
-        err = np.abs(lse - want_lse)[~empty]
+        err = np.abs(lse[~empty] - want_lse[~empty])
         assert (err <= (dw + 4 * EPS * (1 + np.abs(want_lse)))[~empty]).all()
 
 
@@ -254,3 +254,34 @@ def test_attention_int8_scale_of_a_token_without_weight(dctx):
     # (the token's own e^-63.5 x 127 x 60000 is below 2^-60: vmax is the others')
     keep = dict(d, v_scale=np.where(d["v_scale"] == 60000, np.float16(0), d["v_scale"]))
     _check_close(out, lse, q, keep, lens, "int8", 1.0)
+
+
+def test_attention_of_wide_page_tables(dctx):
+    """What bounds the table's width is the work its rows can hold: 256 sequences of 64
+    heads may have rows of 2^20 tokens; a step more than 2^30 of them is refused."""
+    import ctypes
+
+    import torch
+    rng = np.random.default_rng(62)
+    lens, Hq, Hkv, D = [int(n) for n in rng.integers(0, 100, 256)], 64, 8, 64
+    for kv in ("f16", "int8"):
+        d = _cache(rng, kv, lens, Hkv, D)
+        q = rng.normal(0, 1, (256, Hq, D)).astype(np.float16)
+        table = torch.full((256, 1 << 16), 1 << 30, dtype=torch.int32, device="cuda")
+        table[:, :d["table"].shape[1]] = _dev(d["table"])
+        scales = [None if d[n] is None else _dev(d[n]) for n in ("k_scale", "v_scale")]
+        cache = velo_cuda.KvCache(_dev(d["k"]), _dev(d["v"]), table, *scales)
+        out, lse = _attend(dctx, d, q, lens, cache=cache)
+        _check_close(out, lse, q, d, lens, kv)
+    L = velo_cuda.lib()
+    for kv, n_kv, n_head, pages in (("f16", 8, 64, 1 << 15), ("f16", 8, 128, 1 << 15), ("f16", 8, 129 * 8, 3640),
+                                    ("int8", 8, 64, 1 << 16), ("f32", 8, 64, 1 << 14), ("f32", 8, 72, 1 << 13)):
+        # f16, 129 heads a KV head: 9 tiles of 16; f32, 9: two tiles of 8
+        desc = velo_cuda.KvCacheDesc.from_buffer_copy(cache.desc)
+        desc.kv_dtype = {"f16": velo_cuda.KV_F16, "int8": velo_cuda.KV_INT8, "f32": velo_cuda.KV_F32}[kv]
+        desc.n_kv = n_kv
+        for width, message in ((pages, "NULL buffer"), (pages + 2, "2^30")):
+            desc.max_pages = width
+            assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(desc), None, 1 << 20, None, 4096, n_head, 0.0,
+                                                None, None, None, 0) == velo_cuda.ERR_INVALID_ARGUMENT
+            assert message in velo_cuda.last_error(), (kv, width, velo_cuda.last_error())

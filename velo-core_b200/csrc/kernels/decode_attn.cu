@@ -1151,6 +1151,11 @@ int row_tiles(int group, int kv_dtype) {
 
 }  // namespace
 
+int64_t decode_attn_steps(int Hq, int Hkv, int kv_dtype, int max_pages) {
+    const int group = Hq / Hkv, rows = rows_of(row_tiles(group, kv_dtype)), tok = tokens_of(kv_dtype);
+    return (int64_t)Hkv * ((group + rows - 1) / rows) * (((int64_t)max_pages * kPageTokens + tok - 1) / tok);
+}
+
 size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
     // the most that any page type needs
     size_t most = 0;

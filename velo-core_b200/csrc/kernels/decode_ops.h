@@ -59,6 +59,10 @@ struct DecodeAttnArgs {
     void* ws;
     int* err;
 };
+// Steps of work that one sequence filling its page-table row makes; the list of a call
+// is counted in 32 bits.
+constexpr int64_t kDecodeMaxSteps = (int64_t)1 << 30;
+int64_t decode_attn_steps(int Hq, int Hkv, int kv_dtype, int max_pages);
 size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count);
 cudaError_t launch_decode_attention(const DecodeAttnArgs& a, int sm_count, cudaStream_t s);
 

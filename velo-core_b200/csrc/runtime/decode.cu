@@ -163,10 +163,11 @@ int32_t velo_cuda_decode_attention(velo_cuda_ctx* c, const velo_kv_cache* cache,
         return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: B %d outside [0, %d]", B, velo::kDecodeMaxB);
     if (!(scale >= 0.0f) || std::isinf(scale))
         return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: scale must be finite and >= 0");
-    // work is counted in steps of 8 tokens per head at the finest
-    if ((int64_t)B * n_head * 2 * cache->max_pages >= (int64_t)1 << 31)
-        return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: B %d x n_head %d x max_pages %d is too large", B,
-                    n_head, cache->max_pages);
+    const int64_t steps = B * velo::decode_attn_steps(n_head, cache->n_kv, cache->kv_dtype, cache->max_pages);
+    if (steps > velo::kDecodeMaxSteps)
+        return fail(VELO_ERR_INVALID_ARGUMENT,
+                    "decode_attention: %d page-table rows of %d pages are %lld steps of work, above 2^30", B,
+                    cache->max_pages, (long long)steps);
     if (B == 0) return VELO_OK;
     if (!q || !seq_len || !out) return fail(VELO_ERR_INVALID_ARGUMENT, "decode_attention: NULL buffer");
     const int eb = cache->kv_dtype == VELO_KV_F32 ? 4 : 2;
