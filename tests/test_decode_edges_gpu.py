@@ -285,3 +285,28 @@ def test_attention_of_wide_page_tables(dctx):
             assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(desc), None, 1 << 20, None, 4096, n_head, 0.0,
                                                 None, None, None, 0) == velo_cuda.ERR_INVALID_ARGUMENT
             assert message in velo_cuda.last_error(), (kv, width, velo_cuda.last_error())
+
+
+# ------------------------------------------------------------------ log probabilities
+
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+@pytest.mark.parametrize("V", [7, 70001])
+def test_logprobs_of_logits_far_apart(dctx, src, V):
+    """Logits whose difference passes the largest f32, under temperatures that bring
+    the quotient back: a log probability of -6e8 is not -inf, a masked one is."""
+    import torch
+    x = torch.zeros(3, V)
+    x[:, 0], x[:, 1], x[:, 2], x[:, 3] = 3e38, 2e38, -3e38, -np.inf
+    x = x.to({"f32": torch.float32, "bf16": torch.bfloat16}[src])
+    lp, tok = torch.zeros(3, device="cuda"), torch.tensor([1, 2, 3], dtype=torch.int32, device="cuda")
+    ids, tl = torch.zeros(3, min(V, 64), dtype=torch.int32, device="cuda"), torch.zeros(3, min(V, 64), device="cuda")
+    for T in (1e30, 1e25):
+        want = torch.log_softmax(x.double() / T, -1)
+        dctx.token_logprobs(x.cuda(), tok, lp, None, ids, tl, temperature=T)
+        dctx.sync()
+        for got, w in ((lp.cpu().double(), want.gather(1, tok.cpu().long()[:, None])[:, 0]),
+                       (tl.cpu().double(), want.gather(1, ids.cpu().long()))):
+            finite = torch.isfinite(w)
+            assert torch.equal(got[~finite], w[~finite])
+            # 1 / T, its product and the difference: four roundings
+            assert ((got - w)[finite].abs() <= 4 * EPS * w[finite].abs() + 1e-6).all()

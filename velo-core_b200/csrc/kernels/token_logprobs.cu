@@ -488,8 +488,8 @@ __global__ void __launch_bounds__(kThreads, Block<kThreads, kStages>::kPerSm) to
     const float log_z = logf(s.z);
     auto lp = [&](float x) {
         if (log_z != log_z) return log_z;
-        const float d = x - base_of(s.m);
-        return d == -INFINITY ? d : fmaf(d, a.inv_t, -log_z);
+        const float d = 0.5f * x - 0.5f * base_of(s.m);  // halves: the difference may pass the largest f32
+        return d == -INFINITY ? d : fmaf(d, 2.0f * a.inv_t, -log_z);
     };
     if (tid == 0) {
         if (a.logprob) {
