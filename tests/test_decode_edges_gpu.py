@@ -127,6 +127,39 @@ def test_append_flags_starts_that_lose_or_move_tokens(dctx, B):
         run(start.astype(np.int32))
 
 
+def test_append_stores_what_write_kv_stores(dctx):
+    """f16 V rows appended to INT8 and f16 pages: the integers, scales and values that
+    velo_cuda_write_kv stores for the same rows."""
+    import synthetic
+    import torch
+    T, H, D = 50, 2, 128
+    rng = np.random.default_rng(65)
+    v = np.clip(rng.normal(0, 1, (T, H, D)) * np.exp(rng.normal(0, 4, (T, H, 1))), -6e4, 6e4).astype(np.float16)
+    v[3, 1], v[7, 0], v[9, 0, 5] = 0, 2.0 ** -24, 60000
+    meta, tensors = synthetic.llama_q4_model(n_vocab=512, n_embd=256, n_layer=1, n_head=2, n_head_kv=H, n_ff=512, seed=1)
+    for kv in (velo_cuda.KV_INT8, velo_cuda.KV_F16):
+        int8 = kv == velo_cuda.KV_INT8
+        own = velo_cuda.Context(device=0, total_pages=4, max_slots=1, max_pages_per_slot=4, kv_dtype=kv)
+        try:
+            own.load_model(meta, tensors)
+            own.bind_slot(0, np.arange(4, dtype=np.uint32))
+            own.write_kv(0, 0, 0, v, v)
+            stored = own.read_kv(0, 0, 0, T, H, int8=int8)
+        finally:
+            own.close()
+        z = torch.zeros(4, H, 16, D, dtype=torch.int8 if int8 else torch.float16, device="cuda")
+        sc = [torch.zeros(4, H, 16, dtype=torch.float16, device="cuda") for _ in range(2)] if int8 else []
+        cache = velo_cuda.KvCache(z, z.clone(), torch.arange(4, dtype=torch.int32, device="cuda").view(1, 4), *sc)
+        dctx.kv_append(cache, None, _dev(v), _dev(v), _dev(np.zeros(1, np.int32)), None, 10000.0,
+                       seq_start=_dev(np.asarray([0, T], np.int32)))
+        dctx.sync()
+        rows = np.moveaxis(cache.tensors[1].cpu().numpy(), 1, 2).reshape(-1, H, D)[:T]
+        assert np.array_equal(rows, stored[1])
+        if int8:
+            scales = np.moveaxis(cache.tensors[4].cpu().numpy(), 1, 2).reshape(-1, H)[:T]
+            assert np.array_equal(scales.view(np.uint16), stored[3])
+
+
 # ------------------------------------------------------------------ attention
 
 TOKENS = {"f16": 16, "int8": 32, "f32": 8}  # of a step
@@ -285,6 +318,114 @@ def test_attention_of_wide_page_tables(dctx):
             assert L.velo_cuda_decode_attention(dctx.handle, ctypes.byref(desc), None, 1 << 20, None, 4096, n_head, 0.0,
                                                 None, None, None, 0) == velo_cuda.ERR_INVALID_ARGUMENT
             assert message in velo_cuda.last_error(), (kv, width, velo_cuda.last_error())
+
+
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D,lens", ATTN + [(16, 2, 128, [30011, 1]), (32, 8, 64, [1000 + 37 * i % 500 for i in range(40)])])
+def test_attention_close_per_head(dctx, kv, Hq, Hkv, D, lens):
+    rng = np.random.default_rng(Hq * 1000 + D + len(lens) + 1)
+    d = _cache(rng, kv, lens, Hkv, D)
+    q = (rng.normal(0, 1, (len(lens), Hq, D)) * 1.5).astype(np.float32 if kv == "f32" else np.float16)
+    out, lse = _attend(dctx, d, q, lens)
+    _check_close(out, lse, q, d, lens, kv)
+
+
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+@pytest.mark.parametrize("Hq,Hkv,D,lens", [
+    (4, 4, 128, [1, 2, 15, 16, 17, 31, 32, 33, 0, 128, 1000]), (64, 8, 128, [60011]), (32, 32, 128, [203, 4097]),
+    (16, 1, 64, [30011, 5, 20000]), (32, 8, 64, [1000 + 37 * i % 500 for i in range(70)]),
+    (24, 1, 128, [5000, 300]), (18, 2, 64, [7 * i % 300 for i in range(300)])])
+def test_attention_loses_no_token(dctx, kv, Hq, Hkv, D, lens):
+    """Queries of 0 weigh all tokens alike, and token t has a V of 1 in dimension t % D
+    alone: every output is that dimension's share of the tokens, which one token left
+    out or taken twice moves by more than a rounding, wherever the list is cut."""
+    rng = np.random.default_rng(len(lens))
+    d = _cache(rng, kv, lens, Hkv, D)
+    for b, n in enumerate(lens):
+        t = np.arange(n)
+        ids, slots = d["table"][b, t // 16], t % 16
+        d["v"][ids, :, slots] = 0
+        d["v"][ids, :, slots, t % D] = 64 if kv == "int8" else 1
+        if kv == "int8":
+            d["v_scale"][ids, :, slots] = 2.0 ** -6
+    q = np.zeros((len(lens), Hq, D), np.float32 if kv == "f32" else np.float16)
+    out, lse = _attend(dctx, d, q, lens)
+    for b, n in enumerate(lens):
+        share = np.bincount(np.arange(n) % D, minlength=D) / max(n, 1)
+        # sums of ones are exact; the quotient and its product round, as does the output
+        assert (np.abs(out[b] - share) <= _half_step(share, kv != "f32") + 4 * EPS * share).all(), (b, n)
+        assert n or np.isneginf(lse[b]).all()
+        assert n == 0 or (np.abs(lse[b] - np.log(n)) <= 8 * EPS * (1 + np.log(n))).all()
+
+
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+def test_attention_results_beside_the_flag(dctx, kv):
+    """A page outside the pool leaves its tokens out, a length past the row ends with
+    it, a negative one is 0: the flag is set and the results are those."""
+    import torch
+    rng = np.random.default_rng(63)
+    D, Hkv, Hq = 64, 2, 8
+    q = rng.normal(0, 1, (3, Hq, D)).astype(np.float32 if kv == "f32" else np.float16)
+    lens = [64, 64, 57]
+    d = _cache(rng, kv, lens, Hkv, D, spare=0, poison=False)
+    d["table"] = np.ascontiguousarray(d["table"][:, :4])
+    outside = d["k"].shape[0]
+
+    def run(table, n):
+        dd = dict(d, table=table)
+        cache = velo_cuda.KvCache(_dev(dd["k"]), _dev(dd["v"]), _dev(table),
+                                  *(None if d[x] is None else _dev(d[x]) for x in ("k_scale", "v_scale")))
+        out, lse = torch.full((3, Hq, D), 7.0, dtype=_dev(q).dtype, device="cuda"), torch.full((3, Hq), 7.0, device="cuda")
+        ws = torch.empty(dctx.decode_attention_workspace(Hq, Hkv, D), dtype=torch.uint8, device="cuda")
+        dctx.decode_attention(cache, _dev(q), _dev(np.asarray(n, np.int32)), out, ws, lse=lse)
+        with pytest.raises(velo_cuda.VeloError) as e:
+            dctx.sync()
+        assert e.value.status == velo_cuda.ERR_DEVICE_FLAG
+        return out.cpu().numpy(), lse.cpu().numpy()
+
+    def check(got, table, n):
+        _check_close(*got, q, dict(d, table=table), n, kv)
+    check(run(d["table"], [65, -1, 57]), d["table"], [64, 0, 57])
+    check(run(d["table"], [2 ** 31 - 1, -2 ** 31, 57]), d["table"], [64, 0, 57])
+    for lost in range(4):
+        table = d["table"].copy()
+        table[:, lost] = [outside, -1, outside + 3] if lost < 3 else [outside, -1, table[2, 3]]
+        rest = np.delete(d["table"], lost, 1)
+        if lost == 3:  # the last sequence keeps its ragged page
+            got = run(table, lens)
+            want = np.where(np.arange(3)[:, None] < 2, np.pad(rest, ((0, 0), (0, 1))), d["table"])
+            check(got, want, [48, 48, 57])
+        else:
+            check(run(table, lens), rest, [48, 48, 41])
+
+
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+def test_attention_graph_replayed_with_other_lengths(dctx, kv):
+    """One captured call, replayed with lengths that are cut in other places, in
+    fewer ones or not at all."""
+    import torch
+    rng = np.random.default_rng(64)
+    full = [9000, 700, 40]
+    d = _cache(rng, kv, full, 2, 128, poison=False)
+    scales = [None if d[n] is None else _dev(d[n]) for n in ("k_scale", "v_scale")]
+    cache = velo_cuda.KvCache(_dev(d["k"]), _dev(d["v"]), _dev(d["table"]), *scales)
+    q = rng.normal(0, 1, (3, 8, 128)).astype(np.float32 if kv == "f32" else np.float16)
+    qd, nd = _dev(q), torch.tensor([33, 700, 1], dtype=torch.int32, device="cuda")
+    out, lse = torch.zeros_like(qd), torch.zeros(3, 8, device="cuda")
+    ws = torch.empty(dctx.decode_attention_workspace(8, 2, 128), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        dctx.set_stream(torch.cuda.current_stream().cuda_stream)
+        dctx.decode_attention(cache, qd, nd, out, ws, lse=lse)
+    dctx.set_stream(velo_cuda.DEFAULT_STREAM)
+    for lens in ([1, 650, 40], [9000, 0, 17], [0, 0, 0], full, [8999, 1, 0], [16, 16, 16]):
+        nd.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        _check_close(out.cpu().numpy(), lse.cpu().numpy(), q, d, lens, kv)
+    dctx.sync()
 
 
 # ------------------------------------------------------------------ log probabilities
