@@ -8,7 +8,7 @@
 // Work: the batch is one list of units -- a unit is a step of 16 (f16), 32 (int8)
 // or 8 (f32) tokens of one item, an item a (sequence, KV head, tile of query
 // heads) -- cut into equal ranges, one per block, two blocks per SM, whatever the
-// lengths are (and a tail of short ranges, for balance).  An item that a cut runs
+// lengths are (and a tail of short ranges, for balance; decode_cut.cuh).  An item that a cut runs
 // through leaves partial states (max, sum, unnormalised output) in the workspace,
 // which the join kernel, launched as a programmatic dependent, adds in order: no
 // atomics, repeatable bits.  Short items are not cut (the cut moves to their
@@ -44,13 +44,13 @@
 // at the 1500 MHz that the power cap leaves; one of 203 tokens 6.5 us, which is
 // latency: length, page and K/V reads in a row, four steps of a warp, the launch.
 #include <algorithm>
-#include <climits>
 #include <type_traits>
 
 #include "common/elem.cuh"
 #include "common/pdl.cuh"
 #include "common/sm100.cuh"
 #include "common/smem_attr.cuh"
+#include "kernels/decode_cut.cuh"
 #include "kernels/decode_ops.h"
 #include "velo_cuda.h"
 
@@ -63,18 +63,8 @@ using sm100::smem_u32;
 constexpr int kErrSeqLen = 0x6211, kErrPage = 0x6212;
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr int kMinUnits = 4;  // units per block at least: one per warp
-// Items of at most kJoinUnits (below), or of a quarter of a block's range, are never cut.
 constexpr int kRing = 64;  // unit descriptions per warp
 
-// Resident blocks per SM: INT8 pages with at most 8 query heads per KV head need
-// the third (12 warps) to cover the latency of their conversions.
-constexpr int blocks_per_sm(int kv, int R) { return kv == VELO_KV_INT8 && R <= 1 ? 3 : 2; }
-// Query heads of an item: 8 R, or 4 for R = 0, where the tile's columns 4 .. 7 repeat
-// heads 0 .. 3 and carry the remainders of their weights.
-constexpr int rows_of(int R) { return R ? 8 * R : 4; }
-
-constexpr int tokens_of(int kv) { return kv == VELO_KV_F16 ? 16 : kv == VELO_KV_INT8 ? 32 : 8; }
 constexpr int bytes_of(int kv) { return kv == VELO_KV_F16 ? 2 : kv == VELO_KV_INT8 ? 1 : 4; }
 
 // Shared memory of a block; the lengths and the prefix sums follow.
@@ -85,20 +75,12 @@ struct Layout {
     static constexpr int kHalf = kTok * kRow;                   // K, then V
     static constexpr int kStage = 2 * kHalf + (KV == VELO_KV_INT8 ? 4 * kTok : 0);  // + scales
     static constexpr int kStages = (blocks_per_sm(KV, R) == 3 ? 2 : 3) * (128 / D);
-    // What the join costs, in units of a block's time: items are only cut where whole ones would
-    // make some block later by more
-    static constexpr int kJoinUnits = (KV == VELO_KV_F16 ? 24 : KV == VELO_KV_INT8 ? 10 : 12) * (128 / D);
+    static constexpr int kJoinUnits = join_units(KV, D);
     static constexpr int kRings = kWarps * kStages * kStage;
     static constexpr int kStats = kRings + kWarps * kRing * 16;
     static constexpr int kQ = kStats + 3 * kWarps * 16 * 4;     // f32: q, and each warp's weights
     static constexpr int kP = kQ + (KV == VELO_KV_F32 ? 8 * D * 4 : 0);
     static constexpr int kLens = kP + (KV == VELO_KV_F32 ? kWarps * 72 * 4 : 0);
-};
-
-struct Plan {
-    int main, blocks;  // resident blocks; with the tail's, the grid
-    int group;    // query heads per KV head
-    int tiles;    // query-head tiles per KV head
 };
 
 // A partial state: rows x (max, sum), then rows x D of output.
@@ -185,101 +167,6 @@ __device__ __forceinline__ void split_f16(float x, float y, uint32_t& hi, uint32
 // exactly.  The 128 comes off the sums instead of every element.
 __device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return (w & 0x00ff00ffu) ^ 0x00800080u; }
 __device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return even_bytes(w >> 8); }
-
-// a / b, a >= 0 and b > 0: below 2^22 the f32 quotient is within one of it, which the
-// remainder settles (a third of an integer division's latency; a block starts with a
-// chain of these).
-__device__ __forceinline__ int quotient(int a, int b) {
-    if (a >= 1 << 22) return a / b;
-    const int q = (int)__fdividef((float)a, (float)b), r = a - q * b;
-    return q + (r >= b) - (r < 0);
-}
-
-// The largest b with pre[b] <= u.
-__device__ __forceinline__ int find_sequence(const int* pre, int B, int u) {
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= u)
-            lo = mid;
-        else
-            hi = mid;
-    }
-    return lo;
-}
-
-struct Item {
-    int b, it, start, units;  // sequence, item of the sequence, first unit, units
-};
-template <int kTok>
-__device__ __forceinline__ Item item_of(const int* pre, const int* lens, int B, int u) {
-    Item x;
-    x.b = find_sequence(pre, B, u);
-    x.units = (lens[x.b] + kTok - 1) / kTok;
-    x.it = quotient(u - pre[x.b], x.units);
-    x.start = pre[x.b] + x.it * x.units;
-    return x;
-}
-
-// The cut of the list.  `main` blocks, resident from the start, have equal ranges.
-// SMs do not advance alike (range ends of one launch were 30 % apart), so when a
-// range is long the last twelfth of the list is left to short ranges in
-// blocks that start as the first ones end (ragged INT8 batch of 128: 227 -> 207 us at
-// full clock, 236 -> 234 under the power cap; 64 x 4096 f16: 173.7 -> 171).
-constexpr int kTailPerMain = 1, kTailShare = 12;  // blocks; part of the list
-constexpr int kTailUnits = 64;                   // least large range
-constexpr int kTailStates = 24;                  // most short ranges of an item: its join reads that many states
-// n units in k ranges: the first n % k have one unit more.
-struct Share {
-    int n, k, q, r;
-    __device__ __forceinline__ Share(int n_, int k_) : n(n_), k(k_), q(k_ ? quotient(n_, k_) : 0), r(n_ - q * k_) {}
-    __device__ __forceinline__ int at(int c) const { return c * q + min(c, r); }  // first unit of range c
-    __device__ __forceinline__ int range_of(int u) const {
-        return u < r * (q + 1) ? quotient(u, q + 1) : r + quotient(u - r * (q + 1), q);
-    }
-};
-struct Cut {
-    Share big, tail;  // the large ranges, then the short ones
-    bool uncut;       // no item is cut
-    __device__ __forceinline__ int blocks() const { return big.k + tail.k; }
-    __device__ __forceinline__ int total() const { return big.n + tail.n; }
-    __device__ __forceinline__ int at(int c) const { return c <= big.k ? big.at(c) : big.n + tail.at(c - big.k); }
-    __device__ __forceinline__ int block_of(int u) const {
-        return u < big.n ? big.range_of(u) : big.k + tail.range_of(u - big.n);
-    }
-    // Items up to this length are not cut by the start of block c (never more in the tail, so
-    // that moving a cut to an item's start keeps the cuts in order).
-    __device__ __forceinline__ int whole(int c, int least) const {
-        return uncut ? INT_MAX : max(least, (c <= big.k ? big.q : tail.q) / 4);
-    }
-};
-// items: how many there are, longest: units of the longest.
-__device__ __forceinline__ Cut cut_list(const Plan& plan, int total, int items, int longest, int join_units) {
-    const int tail = plan.blocks - plan.main, blocks = min(plan.main, (total + kMinUnits - 1) / kMinUnits);
-    const Share even(total, blocks);
-    // Whole items make the fullest block per * longest - q longer than an equal share at most, and with
-    // several to a block half of the longest on average.  Cutting costs the join and each block an
-    // item's start and end more (128 x 100-600 tokens INT8 48.8 us cut, 45.1 uncut; where blocks would
-    // idle, 16 x 400-800, 15.5 against 17.3).
-    const int per = quotient(items + blocks - 1, blocks);
-    const bool uncut = total > 0 && (2 * ((long long)per * longest - even.q) <= 3 * join_units ||
-                                     (per > 1 && longest <= 2 * join_units));
-    if (tail > 0 && quotient(total, plan.main) >= kTailUnits &&
-        longest <= kTailStates * quotient(total / kTailShare, tail)) {
-        const int n = total / kTailShare;
-        return Cut{Share(total - n, plan.main), Share(n, tail), uncut};
-    }
-    return Cut{even, Share(0, 0), uncut};
-}
-
-// First unit of block c: moved to the start of the item it falls into when that is short.
-template <int kTok>
-__device__ __forceinline__ int cut_at(const int* pre, const int* lens, int B, const Cut& k, int join_units, int c) {
-    const int u = c < k.blocks() ? k.at(c) : k.total();
-    if (c == 0 || u >= k.total()) return u;
-    const Item x = item_of<kTok>(pre, lens, B, u);
-    return x.units <= k.whole(c, join_units) ? x.start : u;
-}
 
 // KV: velo_kv_dtype; D: head_dim; R: tiles of 8 query heads per item (0: half a tile).
 template <int KV, int D, int kTiles>
@@ -1102,11 +989,6 @@ __global__ void __launch_bounds__(kJoinWarps * 32) decode_join_kernel(const Deco
     if (lane == 0 && a.lse) a.lse[(size_t)it.x * a.Hq + head] = L == 0.0f ? -INFINITY : (M + log2f(L)) * kLn2;
 }
 
-int main_blocks(int kv, int R, int sm_count) {
-    return blocks_per_sm(kv, R) * sm_count;
-}
-int all_blocks(int kv, int R, int sm_count) { return main_blocks(kv, R, sm_count) * (1 + kTailPerMain); }
-
 template <int KV, int D, int R>
 cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
     using L = Layout<KV, D, R>;
@@ -1114,25 +996,14 @@ cudaError_t launch_typed(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) 
     const int smem = L::kLens + (2 * a.B + 1) * 4;
     cudaError_t e = ensure_smem(attr, decode_attn_kernel<KV, D, R>, smem);
     if (e != cudaSuccess) return e;
-    Plan p;
-    p.main = main_blocks(KV, R, sm_count);
-    p.blocks = all_blocks(KV, R, sm_count);
-    p.group = a.Hq / a.kv.n_kv;
-    p.tiles = (p.group + rows_of(R) - 1) / rows_of(R);
-    // the tail's blocks only where cut_list can come to use them: enough work in this table,
-    // and enough items that the longest is not above kTailStates short ranges
-    const int most = (a.kv.max_pages * kPageTokens + L::kTok - 1) / L::kTok;  // units of an item at most
-    const long long items = (long long)a.B * a.kv.n_kv * p.tiles;
-    if (items * most < (long long)kTailUnits * p.main ||
-        items * kTailStates < (long long)kTailShare * (p.blocks - p.main))
-        p.blocks = p.main;
+    const Plan p = make_plan(KV, a.Hq / a.kv.n_kv, a.kv.n_kv, a.B, a.kv.max_pages, sm_count);
     e = launch_dependent(decode_attn_kernel<KV, D, R>, dim3(p.blocks), kThreads, smem, 1, s, a, p);
-    if (e != cudaSuccess || most <= L::kJoinUnits) return e;  // no item of this table is ever cut
+    if (e != cudaSuccess || most_units(KV, a.kv.max_pages) <= L::kJoinUnits) return e;  // no item of this table is ever cut
     using Act = typename std::conditional<KV == VELO_KV_F32, float, __half>::type;
     // Few items are cut into many states each: 4 warps per query head.  Otherwise most blocks have
     // nothing to join and only have to leave soon: one of 8 warps for (8 of) an item's heads.
     constexpr int rows = rows_of(R), each = rows < 8 ? rows : 8;
-    if (items <= 16)
+    if ((long long)a.B * a.kv.n_kv * p.tiles <= 16)
         return launch_dependent(decode_join_kernel<Act, D, 4, 1>, dim3(p.blocks, rows), 128, 0, 1, s, a, p, rows);
     return launch_dependent(decode_join_kernel<Act, D, 8, each>, dim3(p.blocks, rows / each), 256, 0, 1, s, a, p, rows);
 }
@@ -1142,18 +1013,11 @@ cudaError_t launch_rows(const DecodeAttnArgs& a, int sm_count, cudaStream_t s) {
     return a.kv.head_dim == 64 ? launch_typed<KV, 64, R>(a, sm_count, s) : launch_typed<KV, 128, R>(a, sm_count, s);
 }
 
-// tiles of 8 query heads per item: f32 items hold 8 heads, the others 4 (half the MMAs
-// for P V), 8 or up to 16
-int row_tiles(int group, int kv_dtype) {
-    if (kv_dtype == VELO_KV_F32) return 1;
-    return group > 8 ? 2 : group > 4 ? 1 : 0;
-}
-
 }  // namespace
 
 int64_t decode_attn_steps(int Hq, int Hkv, int kv_dtype, int max_pages) {
-    const int group = Hq / Hkv, rows = rows_of(row_tiles(group, kv_dtype)), tok = tokens_of(kv_dtype);
-    return (int64_t)Hkv * ((group + rows - 1) / rows) * (((int64_t)max_pages * kPageTokens + tok - 1) / tok);
+    const int group = Hq / Hkv, rows = rows_of(row_tiles(group, kv_dtype));
+    return (int64_t)Hkv * ((group + rows - 1) / rows) * most_units(kv_dtype, max_pages);
 }
 
 size_t decode_attn_workspace(int Hq, int Hkv, int D, int sm_count) {
