@@ -428,6 +428,101 @@ def test_attention_graph_replayed_with_other_lengths(dctx, kv):
     dctx.sync()
 
 
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+@pytest.mark.parametrize("Hq,Hkv", [(8, 2), (16, 2), (32, 2)])
+def test_attention_keeps_nan_to_its_heads(dctx, kv, Hq, Hkv):
+    """A NaN in one head's query, an infinite K and a NaN V in one KV head: the other
+    heads and sequences are as without them, the touched ones hold a NaN."""
+    rng = np.random.default_rng(66)
+    lens, D, group = [700, 33], 64, Hq // Hkv
+    d = _cache(rng, kv, lens, Hkv, D)
+    q = rng.normal(0, 1, (2, Hq, D)).astype(np.float32 if kv == "f32" else np.float16)
+    want = _attend(dctx, d, q, lens)
+    bad = q.copy()
+    bad[0, 1, 7] = np.nan
+    out, lse = _attend(dctx, d, bad, lens)
+    rest = np.ones((2, Hq), bool)
+    rest[0, 1] = False
+    assert np.array_equal(out[rest], want[0][rest]) and np.array_equal(lse[rest], want[1][rest])
+    assert np.isnan(out[0, 1]).all() and np.isnan(lse[0, 1])
+    for name, value in (("k", np.inf), ("v", np.nan)):
+        dd = {n: None if a is None else a.copy() for n, a in d.items()}
+        where = name + "_scale" if kv == "int8" else name
+        dd[where][d["table"][0, 20], 1, 5] = value
+        if kv == "int8":
+            dd[name][d["table"][0, 20], 1, 5, 0] = 1  # (a 0 would already be NaN)
+        out, lse = _attend(dctx, dd, q, lens)
+        rest = np.ones((2, Hq), bool)
+        rest[0, group:] = False
+        assert np.array_equal(out[rest], want[0][rest]) and np.array_equal(lse[rest], want[1][rest])
+        # an infinite K scores +inf, -inf (no weight) or NaN; the head's V is NaN in at least one dimension
+        if name == "v":
+            assert np.isnan(out[0, group:]).any(-1).all() and np.array_equal(lse, want[1])
+
+
+# ------------------------------------------------------------------ far offsets
+
+@pytest.mark.parametrize("kv", ["f16", "int8", "f32"])
+def test_pages_past_32_bits(dctx, kv):
+    """Pools of more than 2^32 elements: the last pages are appended to and read."""
+    import torch
+    Hkv, Hq, D = 8, 32, 128
+    pages = (1 << 32) // (Hkv * 16 * D) + 40
+    dt = {"f16": torch.float16, "int8": torch.int8, "f32": torch.float32}[kv]
+    act = torch.float32 if kv == "f32" else torch.float16
+    pools = [torch.empty(pages, Hkv, 16, D, dtype=dt, device="cuda") for _ in range(2)]
+    sc = [torch.empty(pages, Hkv, 16, dtype=torch.float16, device="cuda") for _ in range(2)] if kv == "int8" else []
+    rng = np.random.default_rng(67)
+    new = [70, 33]
+    ids = np.concatenate((rng.choice(20, 3, replace=False), pages - 1 - rng.choice(20, 5, replace=False)))
+    table = rng.permutation(ids).reshape(2, 4).astype(np.int32)
+    table = np.pad(table, ((0, 0), (0, 1)))
+    table[0, 4], table[1, 3:] = pages - 30, 0
+    cache = velo_cuda.KvCache(*pools, _dev(table), *sc)
+    T = sum(new)
+    x = _dev(rng.normal(0, 1, (T, Hq + 2 * Hkv, D)).astype(np.float32))
+    q, ko, vo = (torch.empty(T, h, D, dtype=act, device="cuda") for h in (Hq, Hkv, Hkv))
+    dctx.kv_append(cache, x[:, :Hq], x[:, Hq:Hq + Hkv], x[:, Hq + Hkv:], _dev(np.zeros(2, np.int32)), q, 10000.0,
+                   seq_start=_dev(np.asarray([0, 70, 103], np.int32)), k_out=ko, v_out=vo)
+    last = q[[69, 102]].contiguous()
+    out, lse = torch.empty_like(last), torch.empty(2, Hq, device="cuda")
+    ws = torch.empty(dctx.decode_attention_workspace(Hq, Hkv, D), dtype=torch.uint8, device="cuda")
+    dctx.decode_attention(cache, last, _dev(np.asarray(new, np.int32)), out, ws, lse=lse)
+    dctx.sync()
+    # the pages in use, copied to a small cache
+    used, at = np.unique(table, return_inverse=True)
+    small = {n: t[_dev(used).long()].cpu().numpy() for n, t in zip(("k", "v", "k_scale", "v_scale"), pools + sc)}
+    small = dict({"k_scale": None, "v_scale": None}, **small, table=at.reshape(table.shape).astype(np.int32))
+    for n, rows in (("k", ko), ("v", vo)):
+        have = small[n][small["table"]].astype(np.float32)  # [2][5][Hkv][16][D]
+        if kv == "int8":
+            have = have * small[n + "_scale"][small["table"]].astype(np.float32)[..., None]
+        have = np.moveaxis(have, 2, 3).reshape(2, -1, Hkv, D).astype(rows.cpu().numpy().dtype)
+        assert np.array_equal(np.concatenate([have[0, :70], have[1, :33]]), rows.cpu().numpy())
+    _check_close(out.cpu().numpy(), lse.cpu().numpy(), last.cpu().numpy(), small, new, kv)
+
+
+@pytest.mark.parametrize("src", ["f32", "bf16"])
+def test_logits_past_32_bits(dctx, src):
+    """Rows further apart than 2^32 elements in all."""
+    import torch
+    M, V, ldl = 17, 5000, (1 << 28) + 1
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16}[src]
+    wide = torch.empty((M - 1) * ldl + V, dtype=dt, device="cuda").as_strided((M, V), (ldl, 1))
+    x = torch.from_numpy(np.random.default_rng(68).normal(0, 3, (M, V)).astype(np.float32)).to(dt).cuda()
+    wide.copy_(x)
+    tok = torch.arange(M, dtype=torch.int32, device="cuda")
+    lp, ids, tl = torch.empty(M, device="cuda"), torch.empty(M, 3, dtype=torch.int32, device="cuda"), torch.empty(M, 3, device="cuda")
+    dctx.token_logprobs(wide, tok, lp, None, ids, tl)
+    dctx.sync()
+    want = torch.log_softmax(x.double(), -1)
+    # (V / 256 + 64) additions, the exponential, arguments of up to 20
+    tol = (V / 256 + 64) * EPS + 2.0 ** -20 + 40 * EPS
+    assert (lp - want.gather(1, tok.long()[:, None])[:, 0]).abs().max() <= tol
+    assert (tl - want.gather(1, ids.long())).abs().max() <= tol
+    assert torch.equal(x.gather(1, ids.long()), x.sort(-1, descending=True).values[:, :3])
+
+
 # ------------------------------------------------------------------ log probabilities
 
 @pytest.mark.parametrize("src", ["f32", "bf16"])
