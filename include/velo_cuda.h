@@ -290,7 +290,8 @@ typedef enum velo_elem { VELO_ELEM_F32 = 0, VELO_ELEM_F16 = 1, VELO_ELEM_BF16 = 
  *   k_pool, v_pool   [pool_pages][n_kv][16][head_dim]: f16 (VELO_KV_F16), int8
  *                    (VELO_KV_INT8, value = q * scale) or f32 (VELO_KV_F32)
  *   k_scale, v_scale [pool_pages][n_kv][16] f16 (INT8 only, else NULL)
- *   page_table       [rows][max_pages] u32 page ids: row b belongs to sequence b
+ *   page_table       [rows][max_pages] u32 page ids: row b belongs to sequence b;
+ *                    max_pages <= 2^26
  * head_dim 64 or 128; at most 65536 heads in these calls. */
 typedef struct velo_kv_cache {
     uint32_t struct_size;  /* sizeof(velo_kv_cache) */
@@ -348,7 +349,7 @@ VELO_API size_t velo_cuda_decode_attention_workspace(velo_cuda_ctx *ctx, int32_t
 /* Attention of one query token per sequence over its cached tokens.  Device
  * memory, asynchronous on the context stream; allocates nothing.
  *   q         [B][n_head][head_dim] (RoPE applied), f32 for f32 pages, else f16;
- *             sequence b's row starts at b * ldq elements
+ *             sequence b's row starts at b * ldq elements, 16-byte aligned (out too)
  *   seq_len   [B] i32: sequence b attends to positions 0 .. seq_len[b] - 1 (its
  *             own new token included, once appended)
  *   scale     of the scores; 0: 1 / sqrt(head_dim)
@@ -375,7 +376,7 @@ VELO_API int32_t velo_cuda_decode_attention(velo_cuda_ctx *ctx, const velo_kv_ca
 /* Log probability of given tokens under softmax(logits / temperature), with the
  * distribution's entropy (nats) and its best alternatives.  Device memory,
  * asynchronous on the context stream.
- *   logits    [M][V] of logits_dtype (velo_elem), row m at m * ldl elements
+ *   logits    [M][V] of logits_dtype (velo_elem), row m at m * ldl elements; V <= 2^24
  *   tokens    [M] u32 (NULL: no logprob)
  *   temperature  in [1e-30, 1e30]
  *   logprob   [M] f32 (with tokens), entropy [M] f32 (or NULL)

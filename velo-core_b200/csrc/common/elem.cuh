@@ -1,4 +1,4 @@
-// elem.cuh -- loads and stores of f32 / f16 / bf16 / int8 elements as f32.
+// elem.cuh -- loads and stores of f32 / f16 / bf16 elements as f32.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -10,7 +10,6 @@ namespace velo {
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_f32(int8_t x) { return (float)x; }
 
 // Eight consecutive elements (16-byte aligned for 2-byte types, two 16-byte
 // loads for f32).

@@ -13,8 +13,8 @@
 // which the join kernel, launched as a programmatic dependent, adds in order: no
 // atomics, repeatable bits.  Short items are not cut (the cut moves to their
 // start), so a batch of short contexts pays no join.  What it pays is each item's start and
-// end, 1.3 us of an SM (256 x 32 tokens, 32/8 heads f16: 24.6 us), so the next item's q is on
-// its way while the warps' states of the last one are joined (29.8 without).
+// end, 1.3 us of an SM (256 x 32 tokens, 32/8 heads f16: 25.3 us), so the next item's q is on
+// its way while the warps' states of the last one are joined (5 us more without).
 //
 // A block's four warps take the units of its range in turn.  Each warp streams
 // its own units through a private ring of 8 KB (head_dim 128) stages filled by
@@ -38,11 +38,12 @@
 //  f32: FFMA, a lane per (token, quarter of the head) for the scores and per 4 (2)
 //   dimensions for the output.  (Exponentials are ex2.approx, 2^-22, in all forms.)
 //
-// Measured on a B200 against 6552 GB/s: 64 sequences of 3900 - 4290 f16 tokens, 64/8
-// heads, 168 us back to back (0.98); one of 100003 tokens 73 us (0.86: start-up and
-// join); 128 ragged INT8 sequences, 32/8 heads, 207 us at full clock (0.86), 220 - 235
-// at the 1500 MHz that the power cap leaves; one of 203 tokens 6.5 us, which is
-// latency: length, page and K/V reads in a row, four steps of a warp, the launch.
+// Measured on a B200 against 6552 GB/s, device time back to back: 64 sequences of 3900 - 4290
+// f16 tokens, 64/8 heads, 174.6 us (0.94); one of 100003 tokens 73.8 us (0.85: start-up and
+// join); 128 ragged INT8 sequences, 32/8 heads, 229 us (0.78) at the 1500 MHz that the power cap
+// leaves, 201 in a short burst; one of 203 tokens 6.7 us, which is latency: length,
+// page and K/V reads in a row, four steps of a warp, the launch.  The step's own unit of the
+// weights costs 1.6 us of the 174.6 and 0.2 of the 6.7.
 #include <algorithm>
 #include <type_traits>
 

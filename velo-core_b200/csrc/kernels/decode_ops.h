@@ -44,7 +44,7 @@ struct KvAppendArgs {
     int* err;
     RopeTurns turns;
 };
-cudaError_t launch_kv_append(const KvAppendArgs& a, int sm_count, cudaStream_t s);
+cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s);
 
 constexpr int kDecodeMaxB = 4096;
 struct DecodeAttnArgs {

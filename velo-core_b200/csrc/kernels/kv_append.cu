@@ -13,12 +13,12 @@
 // shared memory, then a thread takes 8 rotation pairs of a head, in equal rounds
 // when there are more than 256 such items.  A block's time is mostly the latency of
 // finding its place (sequence, page, angles) and its rows, so six blocks per SM
-// matter more than loads moved up within one (measured: 13.5 us against 11.6 for
-// 2048 tokens of INT8 pages).
+// matter more than loads moved up within one (2048 tokens of INT8 pages took 13.5 us with
+// them and 11.6 without, before the sine and cosine were taken in 64 bits).
 //
 // Measured on a B200 against 6552 GB/s: 8533 prompt tokens of 32/32 heads, f32 to f16
-// pages, 95 us (1.0); 2048 tokens of 32/8 heads, bf16 to INT8, 12.2 us (0.68, latency);
-// 64 single tokens of 64/8 heads 3.2 us.
+// pages, 96 us (1.0); 2048 tokens of 32/8 heads, bf16 to INT8, 12.4 us (0.67, latency);
+// 64 single tokens of 64/8 heads 3.3 us.
 #include <algorithm>
 
 #include "common/elem.cuh"
@@ -212,7 +212,7 @@ cudaError_t launch_from(const KvAppendArgs& a, cudaStream_t s) {
 
 }  // namespace
 
-cudaError_t launch_kv_append(const KvAppendArgs& a, int, cudaStream_t s) {
+cudaError_t launch_kv_append(const KvAppendArgs& a, cudaStream_t s) {
     if (a.in_dtype == VELO_ELEM_F32) return launch_from<float>(a, s);
     if (a.in_dtype == VELO_ELEM_F16) return launch_from<__half>(a, s);
     return launch_from<__nv_bfloat16>(a, s);

@@ -139,7 +139,7 @@ int32_t velo_cuda_kv_append(velo_cuda_ctx* c, const velo_kv_cache* cache, const 
     a.v_out = in->v_out;
     a.err = c->err_flag;
     a.turns = rope_turns(c, in->freq_base, D);
-    VELO_CUDA_TRY(velo::launch_kv_append(a, c->sm_count, c->stream));
+    VELO_CUDA_TRY(velo::launch_kv_append(a, c->stream));
     return VELO_OK;
 }
 
