@@ -163,7 +163,12 @@ __device__ __forceinline__ void add_two(float2& z, float2& y, float x0, float x1
     y = __ffma2_rn(e, u, y);
 }
 
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+// The .aligned forms take a warp's threads together, which branches on the thread before them
+// do not promise by themselves.
+__device__ __forceinline__ void cluster_arrive() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t map_to_first(uint32_t addr) {
     uint32_t r;
